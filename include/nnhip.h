@@ -381,6 +381,98 @@ int nnhip_spec_accept(nnhip_ctx *ctx, const float *tlogits,
                       int k, int V, float temperature, int32_t *n_accept,
                       int32_t *next_tok);
 
+/* ---- paged int8 KV cache (dev buffers, stream-ordered) ---------------------
+ * Requests of different lengths over one pool of blocks.  No counterpart in
+ * the reference, whose caches hold one sequence each (layer.hpp:212-230): the
+ * operators below are the RoPE append, the attention and the cache readers of
+ * MultiHeadAttention::forward (layer.cpp:593-994) for ragged batches, with a
+ * scale for each block and head where KVCache(true) has one for each row.
+ *
+ * Pool: num_blocks blocks of block_size tokens (16, 32, 64 or 128; at most
+ * 2^31 - 1 slots in all).
+ *   codes  [num_blocks][2][Hkv][block_size * D] int8, aligned to 16 bytes:
+ *          k (index 0) as [block_size][D], v (index 1) as [D][block_size]
+ *   scales [num_blocks][2][Hkv] fp32; a cached value is code * scale
+ * D is 32, 64 or 128 (others: NNHIP_EUNSUPPORTED), H a multiple of Hkv.  Slot
+ * s is token s % block_size of block s / block_size.  No buffer written by a
+ * call may overlap another of its buffers.  Requests may share blocks that
+ * are only read; blocks that a call writes belong to one request each.
+ *
+ * nnhip_block_tables: a step's block tables and slot maps from request
+ * lengths.  Request b of B (at most 4096) keeps cached[b] tokens and adds
+ * added[b]; it then holds ceil((cached + added) / block_size) blocks, the
+ * first entries of its row of tables [B][max_blocks].  held [B] is the number
+ * of blocks it held before (updated).  Missing blocks are taken from the stack
+ * free_list [num_blocks], whose first free_count [1] entries are the free
+ * blocks (both updated), surplus ones go back to it: a shorter cached (drafts
+ * that were rejected) or 0, 0 (a request that ended) frees blocks.  Returned
+ * blocks go on top of the stack, the first request's first one uppermost, and
+ * the taken ones come off it in the order of requests and entries, so a step
+ * that is taken back restores the stack.  Entries of tables behind a request's
+ * blocks and of free_list behind free_count stay as they were.
+ * Written: row_start [B + 1], the sums of added (request b has rows
+ * row_start[b] .. row_start[b + 1] - 1); lens [B] = cached + added; per row,
+ * of T that pos and slots have room for, its position in the request and its
+ * slot, -1 in both behind the last row; status [1]: 0, or why nothing was
+ * changed, with row_start and lens 0 and every row -1, so that the calls that
+ * follow find no rows: the first that holds of 1 a length is negative, 2 a
+ * request needs more than max_blocks blocks, 3 there are more than T rows, 5
+ * held or free_count contradict the pool, 4 too few blocks are free.  T may be
+ * 0, with pos and slots NULL. */
+int nnhip_block_tables(nnhip_ctx *ctx, int B, const int32_t *cached,
+                       const int32_t *added, int block_size, int max_blocks,
+                       int32_t *tables, int32_t *held, int num_blocks,
+                       int32_t *free_list, int32_t *free_count, int T,
+                       int32_t *row_start, int32_t *lens, int32_t *pos,
+                       int32_t *slots, int32_t *status);
+/* RoPE on q and k of qkv [T][q: H heads | k: Hkv | v: Hkv] rows of D, pairs
+ * (2j, 2j + 1) turned by cos_t / sin_t [n_pos][D / 2] at pos[t] (both NULL: the
+ * reference's angles, tensor.cpp:1141-1173), q_out [T][H * D], then k and v
+ * into slots[t] of the pool.  The rows of one block lie within block_size rows
+ * of one another, in any order (where several name a slot, the last counts).
+ * The scale of a (block, k or v, head) is the smallest power of two 2^e, e >=
+ * -126, with max|x| <= 127 * 2^e over the rows it is given (0 when they are all
+ * 0), codes are x / scale rounded to the nearest, ties to even.  A call that
+ * brings a block's first token starts the block anew; one whose rows begin
+ * behind older tokens keeps the scale or raises it, the older codes are then
+ * rescaled and rounded again.  Tokens of the block that are not older and have
+ * no row stay as they were.  A value that is no finite number makes the scale of its
+ * (block, k or v, head) NaN, and with it every result that reads the block,
+ * until the block is started anew.  A row whose slot is outside the pool (-1:
+ * padding) or whose position is outside [0, n_pos) is skipped, its q_out row
+ * stays as it was.  qkv and q_out aligned to 16 bytes, cos_t and sin_t to 8.
+ * T may be 0. */
+int nnhip_rope_kv_append_paged_q8(nnhip_ctx *ctx, const float *qkv, int T,
+                                  int H, int Hkv, int D, const int32_t *pos,
+                                  const int32_t *slots, const float *cos_t,
+                                  const float *sin_t, int n_pos, float *q_out,
+                                  int8_t *codes, float *scales,
+                                  int block_size, int num_blocks);
+/* Causal attention of q rows [T][H * D] over the pool: request b has rows
+ * row_start[b] .. row_start[b + 1] - 1, the last of its lens[b] cached tokens,
+ * so row i of n sees tokens 0 .. lens[b] - n + i, at the blocks that row b of
+ * tables [B][max_blocks] names; scores are q . k / sqrt(D).  out [T][H * D]; a
+ * row that sees no token gives zeros, rows of no request stay as they were.
+ * Blocks beyond a request's tokens are not read, tokens that a row does not
+ * see have no part in it whatever they hold.  A table entry outside the pool
+ * where a token is seen makes the row NaN; lens is cut to max_blocks blocks
+ * and row_start to [0, T].  q and out aligned to 16 bytes; B at most 4096; T
+ * may be 0.  A row's last bits depend on the batch it is in (the kernel and
+ * the split of the keys go by the launch's sizes). */
+int nnhip_attention_paged_q8(nnhip_ctx *ctx, const float *q, int T,
+                             const int8_t *codes, const float *scales,
+                             int block_size, int num_blocks,
+                             const int32_t *tables, int max_blocks,
+                             const int32_t *row_start, const int32_t *lens,
+                             int B, int H, int Hkv, int D, float *out);
+/* KVCache::k / KVCache::v (layer.hpp:213-214) of T slots, in any order: k and
+ * v [T][Hkv][D] fp32 = code * scale.  Rows whose slot is outside the pool stay
+ * as they were.  k and v aligned to 16 bytes; T may be 0. */
+int nnhip_kv_read_paged_q8(nnhip_ctx *ctx, const int8_t *codes,
+                           const float *scales, int block_size,
+                           int num_blocks, const int32_t *slots, int T,
+                           int Hkv, int D, float *k, float *v);
+
 /* ---- ExecutionBackend ops (dev buffers, stream-ordered) -------------------
  * The strided fp32 ops of the reference's backend interface
  * (include/backend/backend.hpp:35-220) with CpuBackend's semantics

@@ -627,6 +627,8 @@ int nnhip_linear_limb_totals(nnhip_ctx *ctx, const float *x, int rows, int K,
   });
 }
 
+}  // extern "C"
+
 // RoPE factors for positions [0, cap) by the reference's float formula
 // (tensor.cpp:1141-1173): theta = pow(10000, -2j/D), omega = pos * theta.
 static void rope_tables(int cap, int D, std::vector<float> &hc,
@@ -647,7 +649,7 @@ static void rope_tables(int cap, int D, std::vector<float> &hc,
 // built once per width (and again only when a call needs more positions,
 // after the stream has drained), so the append entry points neither compute
 // tables nor synchronise per call.
-static const nnhip_ctx::Rope &ctx_rope(nnhip_ctx *ctx, int cap, int D) {
+const nnhip_ctx::Rope &nnhip::ctx_rope(nnhip_ctx *ctx, int cap, int D) {
   nnhip_ctx::Rope *slot = nullptr;
   for (auto &r : ctx->rope)
     if (r.D == D) { slot = &r; break; }
@@ -673,6 +675,8 @@ static const nnhip_ctx::Rope &ctx_rope(nnhip_ctx *ctx, int cap, int D) {
   return *slot;
 }
 
+extern "C" {
+
 int nnhip_rope_kv_append(nnhip_ctx *ctx, const float *qkv, int B, int S,
                          int H, int D, const int32_t *pos, float *q_out,
                          float *kcache, float *vcache, int cap) {
@@ -681,7 +685,7 @@ int nnhip_rope_kv_append(nnhip_ctx *ctx, const float *qkv, int B, int S,
             H > 0 && D > 0 && D % 2 == 0 && cap > 0,
         "nnhip_rope_kv_append: bad argument");
     hipStream_t st = ctx->c.stream;
-    const nnhip_ctx::Rope &rt = ctx_rope(ctx, cap, D);
+    const nnhip_ctx::Rope &rt = nnhip::ctx_rope(ctx, cap, D);
     nnhip::launch_rope_kv(st, qkv, B, S, H, D, pos, 0, nullptr, rt.c.p, rt.s.p,
                           q_out, kcache, vcache, cap, (int64_t)H * cap * D);
   });
@@ -696,7 +700,7 @@ int nnhip_rope_kv_append_gqa(nnhip_ctx *ctx, const float *qkv, int B, int S,
             H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0 && D % 2 == 0 && cap > 0,
         "nnhip_rope_kv_append_gqa: bad argument");
     hipStream_t st = ctx->c.stream;
-    const nnhip_ctx::Rope &rt = ctx_rope(ctx, cap, D);
+    const nnhip_ctx::Rope &rt = nnhip::ctx_rope(ctx, cap, D);
     nnhip::launch_rope_kv(st, qkv, B, S, H, D, pos, 0, nullptr, rt.c.p, rt.s.p,
                           q_out, kcache, vcache, cap, (int64_t)Hkv * cap * D,
                           Hkv);
@@ -733,7 +737,7 @@ int nnhip_rope_kv_append_q8(nnhip_ctx *ctx, const float *qkv, int B, int S,
             B > 0 && S > 0 && H > 0 && D > 0 && D % 2 == 0 && D <= 64 && cap > 0,
         "nnhip_rope_kv_append_q8: bad argument");
     hipStream_t st = ctx->c.stream;
-    const nnhip_ctx::Rope &rt = ctx_rope(ctx, cap, D);
+    const nnhip_ctx::Rope &rt = nnhip::ctx_rope(ctx, cap, D);
     nnhip::launch_rope_kv_q8(st, qkv, B, S, H, D, pos, 0, nullptr, rt.c.p,
                              rt.s.p, q_out, kcodes, kscales, vcodes, vscales,
                              cap, (int64_t)H * cap * D, (int64_t)H * cap);

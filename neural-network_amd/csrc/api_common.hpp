@@ -25,6 +25,8 @@ struct nnhip_ctx {
     nnhip::DevBuf<float> c, s;
   } rope[4];
   nnhip::DevBuf<float> part;
+  // the ticket of nnhip_block_tables' workgroups: zero between calls
+  nnhip::DevBuf<unsigned> ticket;
   // nnhip_spec_accept's state and scratch, kept for the next call of the
   // same (B, k, V) (every call resets the state and synchronizes the stream)
   std::unique_ptr<nnhip::AcceptRows> accept;
@@ -45,6 +47,9 @@ void set_last_error(const std::string &msg);
 void noalloc_setup(int device);
 // gives up the scratch array a destroyed context owned
 void noalloc_release(const nnhip_ctx *ctx);
+
+// the context's RoPE tables for head width D covering positions [0, cap)
+const nnhip_ctx::Rope &ctx_rope(nnhip_ctx *ctx, int cap, int D);
 
 template <typename F>
 int guard(F &&f) {

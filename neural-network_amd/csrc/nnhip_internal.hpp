@@ -3,6 +3,7 @@
 #pragma once
 
 #include "dispatch.hpp"
+#include "paged.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -464,6 +465,23 @@ void launch_rope_kv_q8(hipStream_t st, const float *qkv, int B, int S, int H,
                        const float *sinb, float *qrot, int8_t *kq, float *ks,
                        int8_t *vq, float *vs, int cap, int64_t seq_stride,
                        int64_t sc_stride);
+// The paged int8 KV cache (paged.hpp has its layout and index rules; paged.hip).
+// ticket: one zero on the device, left zero.
+void launch_block_tables(hipStream_t st, int B, const int32_t *cached, const int32_t *added,
+                         int lbs, int max_blocks, int32_t *tables, int32_t *held, int blocks,
+                         int32_t *free_list, int32_t *free_count, int T, int32_t *row_start,
+                         int32_t *lens, int32_t *pos, int32_t *slots, int32_t *status,
+                         unsigned *ticket);
+void launch_rope_append_paged(hipStream_t st, const float *qkv, int T, int H, const PagedPool &p,
+                              const int32_t *pos, const int32_t *slots, const float *cosb,
+                              const float *sinb, int n_pos, float *q_out, int8_t *codes,
+                              float *scales);
+void launch_kv_read_paged(hipStream_t st, const int8_t *codes, const float *scales,
+                          const PagedPool &p, const int32_t *slots, int T, float *k, float *v);
+void launch_attention_paged(hipStream_t st, const float *q, int T, const int8_t *codes,
+                            const float *scales, const PagedPool &p, const int32_t *tables,
+                            int max_blocks, const int32_t *row_start, const int32_t *lens, int B,
+                            int H, float *out);
 // K / V rows an attention launch reads: fp32 rows, or int8 codes with one
 // fp32 scale per (head, position) row (KVCache(quantized=true),
 // layer.hpp:212-230).  Rows [B][Hkv][cap][D], seq_stride elements apart

@@ -131,6 +131,14 @@ SIGNATURES = {
     "nnhip_sample_rows": [_vp, _vp, _i, _i, _f, _i, _f, _vp, _vp, _vp],
     "nnhip_spec_accept": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp,
                           _vp],
+    "nnhip_block_tables": [_vp, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp,
+                           _i, _vp, _vp, _vp, _vp, _vp],
+    "nnhip_rope_kv_append_paged_q8": [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp,
+                                      _vp, _i, _vp, _vp, _vp, _i, _i],
+    "nnhip_attention_paged_q8": [_vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _vp,
+                                 _vp, _i, _i, _i, _i, _vp],
+    "nnhip_kv_read_paged_q8": [_vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _vp,
+                               _vp],
     "nnhip_binary_f32": [_vp, _i, C.POINTER(View), C.POINTER(View),
                          C.POINTER(View)],
     "nnhip_unary_f32": [_vp, _i, C.POINTER(View), C.POINTER(View)],
@@ -446,3 +454,87 @@ class KVCache:
         call("nnhip_kvcache_read_q8", self.h, layer, b, ptr(kq), ptr(ks),
              ptr(vq), ptr(vs))
         return kq, ks, vq, vs
+
+
+class PagedKVCache:
+    """A pool of `num_blocks` int8 KV blocks for each of `layers` attention
+    layers, and the block tables of `batch` requests: step() plans a step's
+    rows from the requests' lengths, append() and attention() run one layer's
+    part of it."""
+
+    def __init__(self, ctx, batch, max_blocks, num_blocks, block_size, H, Hkv,
+                 D, layers=1):
+        self.ctx, self.batch, self.max_blocks = ctx, batch, max_blocks
+        self.num_blocks, self.block_size = num_blocks, block_size
+        self.H, self.Hkv, self.D = H, Hkv, D
+        i32 = np.int32
+        self.tables = ctx.array(np.full((batch, max_blocks), -1, i32))
+        self.held = ctx.array(np.zeros(batch, i32))
+        self.free_list = ctx.array(np.arange(num_blocks, dtype=i32)[::-1])
+        self.free_count = ctx.array(np.array([num_blocks], i32))
+        self.codes = [ctx.array(np.zeros((num_blocks, 2, Hkv, block_size * D),
+                                         np.int8)) for _ in range(layers)]
+        self.scales = [ctx.array(np.zeros((num_blocks, 2, Hkv), np.float32))
+                       for _ in range(layers)]
+        self.row_start = ctx.array(np.zeros(batch + 1, i32))
+        self.lens = ctx.array(np.zeros(batch, i32))
+        self.status = ctx.array(np.zeros(1, i32))
+        self.pos = self.slots = None
+        self.T = 0
+
+    def step(self, cached, added, rows=None):
+        """Blocks, positions and slots of a step in which request b keeps
+        cached[b] tokens and adds added[b]; `rows`: rows of the step's
+        buffers (default: as many as are added)."""
+        cached = np.ascontiguousarray(cached, np.int32)
+        added = np.ascontiguousarray(added, np.int32)
+        assert cached.shape == added.shape == (self.batch,)
+        T = int(added.sum()) if rows is None else rows
+        c, a = self.ctx.array(cached), self.ctx.array(added)
+        self.ctx.sync()         # calls that read the last step's buffers
+        self.pos = self.ctx.array(shape=(max(T, 1),), dtype=np.int32)
+        self.slots = self.ctx.array(shape=(max(T, 1),), dtype=np.int32)
+        self.T = T
+        call("nnhip_block_tables", self.ctx.h, self.batch, c.p, a.p,
+             self.block_size, self.max_blocks, self.tables.p, self.held.p,
+             self.num_blocks, self.free_list.p, self.free_count.p, T,
+             self.row_start.p, self.lens.p, self.pos.p, self.slots.p,
+             self.status.p)
+        st = int(self.status.numpy()[0])
+        if st:
+            raise NNHipError(ECAPACITY if st in (2, 4) else EARG,
+                             "PagedKVCache.step: " + (
+                                 "a length is negative",
+                                 "a request needs more than max_blocks blocks",
+                                 "more rows than the buffers hold",
+                                 "too few blocks are free",
+                                 "held or free_count contradict the pool",
+                             )[st - 1])
+
+    def append(self, qkv, q_out, n_pos, cos=None, sin=None, layer=0):
+        """RoPE on the step's rows, k and v into their slots; n_pos: positions
+        of cos and sin, or of the reference's angles without them."""
+        call("nnhip_rope_kv_append_paged_q8", self.ctx.h, qkv.p, self.T,
+             self.H, self.Hkv, self.D, self.pos.p, self.slots.p,
+             cos.p if cos is not None else None,
+             sin.p if sin is not None else None, n_pos, q_out.p,
+             self.codes[layer].p, self.scales[layer].p, self.block_size,
+             self.num_blocks)
+
+    def attention(self, q, out, layer=0):
+        call("nnhip_attention_paged_q8", self.ctx.h, q.p, self.T,
+             self.codes[layer].p, self.scales[layer].p, self.block_size,
+             self.num_blocks, self.tables.p, self.max_blocks,
+             self.row_start.p, self.lens.p, self.batch, self.H, self.Hkv,
+             self.D, out.p)
+
+    def read(self, slots, layer=0):
+        """k and v [n][Hkv][D] of n slots (host)."""
+        s = self.ctx.array(np.ascontiguousarray(slots, np.int32))
+        n = s.shape[0]
+        k = self.ctx.array(np.zeros((n, self.Hkv, self.D), np.float32))
+        v = self.ctx.array(np.zeros((n, self.Hkv, self.D), np.float32))
+        call("nnhip_kv_read_paged_q8", self.ctx.h, self.codes[layer].p,
+             self.scales[layer].p, self.block_size, self.num_blocks, s.p, n,
+             self.Hkv, self.D, k.p, v.p)
+        return k.numpy(), v.numpy()
