@@ -392,7 +392,8 @@ int nnhip_spec_accept(nnhip_ctx *ctx, const float *tlogits,
  * 2^31 - 1 slots in all).
  *   codes  [num_blocks][2][Hkv][block_size * D] int8, aligned to 16 bytes:
  *          k (index 0) as [block_size][D], v (index 1) as [D][block_size]
- *   scales [num_blocks][2][Hkv] fp32; a cached value is code * scale
+ *   scales [num_blocks][2][Hkv] fp32, not negative; a cached value is code *
+ *          scale (in the attention a scale below 2^-126 counts as 0)
  * D is 32, 64 or 128 (others: NNHIP_EUNSUPPORTED), H a multiple of Hkv.  Slot
  * s is token s % block_size of block s / block_size.  No buffer written by a
  * call may overlap another of its buffers.  Requests may share blocks that

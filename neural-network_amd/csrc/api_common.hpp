@@ -25,8 +25,11 @@ struct nnhip_ctx {
     nnhip::DevBuf<float> c, s;
   } rope[4];
   nnhip::DevBuf<float> part;
-  // the ticket of nnhip_block_tables' workgroups: zero between calls
-  nnhip::DevBuf<unsigned> ticket;
+  // the tickets of nnhip_block_tables' workgroups and of
+  // nnhip_attention_paged_q8's units: zero between calls; the latter's partial
+  // results
+  nnhip::DevBuf<unsigned> ticket, paged_tickets;
+  nnhip::DevBuf<float> paged_part;
   // nnhip_spec_accept's state and scratch, kept for the next call of the
   // same (B, k, V) (every call resets the state and synchronizes the stream)
   std::unique_ptr<nnhip::AcceptRows> accept;

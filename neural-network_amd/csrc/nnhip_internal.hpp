@@ -465,7 +465,8 @@ void launch_rope_kv_q8(hipStream_t st, const float *qkv, int B, int S, int H,
                        const float *sinb, float *qrot, int8_t *kq, float *ks,
                        int8_t *vq, float *vs, int cap, int64_t seq_stride,
                        int64_t sc_stride);
-// The paged int8 KV cache (paged.hpp has its layout and index rules; paged.hip).
+// The paged int8 KV cache (paged.hpp has its layout and index rules; paged.hip,
+// paged_attention.hip).
 // ticket: one zero on the device, left zero.
 void launch_block_tables(hipStream_t st, int B, const int32_t *cached, const int32_t *added,
                          int lbs, int max_blocks, int32_t *tables, int32_t *held, int blocks,
@@ -481,7 +482,10 @@ void launch_kv_read_paged(hipStream_t st, const int8_t *codes, const float *scal
 void launch_attention_paged(hipStream_t st, const float *q, int T, const int8_t *codes,
                             const float *scales, const PagedPool &p, const int32_t *tables,
                             int max_blocks, const int32_t *row_start, const int32_t *lens, int B,
-                            int H, float *out);
+                            int H, float *out, float *part, unsigned *tickets);
+// floats of `part` and (zero, left zero) entries of `tickets` that it needs
+int64_t attention_paged_part_elems(int D);
+int attention_paged_tickets();
 // K / V rows an attention launch reads: fp32 rows, or int8 codes with one
 // fp32 scale per (head, position) row (KVCache(quantized=true),
 // layer.hpp:212-230).  Rows [B][Hkv][cap][D], seq_stride elements apart

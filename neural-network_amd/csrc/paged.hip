@@ -1,5 +1,6 @@
 // The paged int8 KV cache: block tables and slot maps from request lengths,
-// RoPE + append into blocks, attention over them, and reading rows back.
+// RoPE + append into blocks, and reading rows back (attention over them:
+// paged_attention.hip).
 #include "nnhip_internal.hpp"
 
 #include <algorithm>
@@ -337,75 +338,6 @@ __global__ __launch_bounds__(256) void kv_read_paged_kernel(
   }
 }
 
-// ---------------------------------------------------------------------------
-// Attention: a wave per (row, head), 64 keys at a time.
-__global__ __launch_bounds__(64) void attn_paged_kernel(
-    const float *__restrict__ q, int T, const int8_t *__restrict__ codes,
-    const float *__restrict__ scales, PagedPool p, const int32_t *__restrict__ tables,
-    int max_blocks, const int32_t *__restrict__ row_start, const int32_t *__restrict__ lens, int B,
-    int H, float *__restrict__ out) {
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, D = p.D;
-  int b = 0;
-  RowRange rr{0, 0};
-  for (; b < B; ++b) {
-    rr = request_rows(row_start, b, T);
-    if (t >= rr.first && t < rr.last) break;
-  }
-  if (b == B) return;
-  const int hk = h / (H / p.Hkv);
-  const int64_t len = request_len(lens[b], max_blocks, p.lbs);
-  const int64_t see = len - (rr.last - rr.first) + (t - rr.first) + 1;  // visible keys
-  __shared__ float s_q[128], s_p[64];
-  __shared__ int s_blk[64];
-  for (int d = lane; d < D; d += 64) s_q[d] = q[((int64_t)t * H + h) * D + d] * rsqrtf((float)D);
-  __syncthreads();
-  float m = -INFINITY, l = 0, o[2] = {0, 0};
-  for (int64_t j0 = 0; j0 < see; j0 += 64) {
-    const int64_t j = j0 + lane;
-    float s = -INFINITY;
-    int blk = 0;
-    if (j < see) {
-      blk = tables[(int64_t)b * max_blocks + (j >> p.lbs)];
-      if (!block_ok(blk, p.blocks)) {
-        s = NAN;
-        blk = -1;
-      } else {
-        const int8_t *kc = codes + head_offset(p, blk, 0, hk) + (j & (p.bs - 1)) * D;
-        float x = 0;
-        for (int d = 0; d < D; ++d) x = fmaf(s_q[d], (float)kc[d], x);
-        s = x * scales[scale_offset(p, blk, 0, hk)];
-      }
-    }
-    float mx = s;
-    for (int o2 = 32; o2; o2 >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o2, 64));
-    const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : __expf(m - mn);
-    const float e = j < see ? expf(s - mn) : 0.f;
-    float sum = e;
-    for (int o2 = 32; o2; o2 >>= 1) sum += __shfl_xor(sum, o2, 64);
-    l = l * f + sum;
-    m = mn;
-    s_p[lane] = blk < 0 ? NAN : j < see ? e * scales[scale_offset(p, blk, 1, hk)] : 0.f;
-    s_blk[lane] = blk;
-    __syncthreads();
-    for (int i = 0; i < 2; ++i) {
-      const int d = lane + 64 * i;
-      if (d >= D) continue;
-      float acc = o[i] * f;
-      for (int k = 0; k < 64 && j0 + k < see; ++k) {
-        const int bk = s_blk[k];
-        const float code = bk < 0 ? 0.f
-            : (float)codes[head_offset(p, bk, 1, hk) + (d << p.lbs) + ((j0 + k) & (p.bs - 1))];
-        acc = fmaf(s_p[k], code, acc);
-      }
-      o[i] = acc;
-    }
-    __syncthreads();
-  }
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < D)
-      out[((int64_t)t * H + h) * D + lane + 64 * i] = see > 0 ? o[i] / l : 0.f;
-}
-
 }  // namespace
 
 void launch_block_tables(hipStream_t st, int B, const int32_t *cached, const int32_t *added,
@@ -435,15 +367,6 @@ void launch_kv_read_paged(hipStream_t st, const int8_t *codes, const float *scal
   const int64_t units = (int64_t)T * p.Hkv;
   hipLaunchKernelGGL(kv_read_paged_kernel, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st,
                      codes, scales, p, slots, T, k, v);
-  NNHIP_CHECK(hipGetLastError());
-}
-
-void launch_attention_paged(hipStream_t st, const float *q, int T, const int8_t *codes,
-                            const float *scales, const PagedPool &p, const int32_t *tables,
-                            int max_blocks, const int32_t *row_start, const int32_t *lens, int B,
-                            int H, float *out) {
-  hipLaunchKernelGGL(attn_paged_kernel, dim3(T, H), dim3(64), 0, st, q, T, codes, scales, p, tables,
-                     max_blocks, row_start, lens, B, H, out);
   NNHIP_CHECK(hipGetLastError());
 }
 

@@ -38,6 +38,13 @@ nnhip::PagedPool pool_of(int block_size, int num_blocks, int Hkv, int D, const v
   return p;
 }
 
+// n zeros in `b`, which is set only once they are under way.
+void zeroed(nnhip::DevBuf<unsigned> &b, size_t n, hipStream_t st) {
+  nnhip::DevBuf<unsigned> z(n);
+  NNHIP_CHECK(hipMemsetAsync(z.p, 0, z.bytes(), st));
+  b = std::move(z);
+}
+
 void check_heads(int H, int Hkv, const char *what) {
   REQ(H > 0 && H <= 65535 && H % Hkv == 0, std::string(what) + ": H must be a multiple of Hkv");
 }
@@ -65,10 +72,7 @@ int nnhip_block_tables(nnhip_ctx *ctx, int B, const int32_t *cached, const int32
         "nnhip_block_tables: NULL argument");
     set_device(ctx);
     hipStream_t st = ctx->c.stream;
-    if (!ctx->ticket.p) {
-      ctx->ticket.alloc(1);
-      NNHIP_CHECK(hipMemsetAsync(ctx->ticket.p, 0, ctx->ticket.bytes(), st));
-    }
+    if (!ctx->ticket.p) zeroed(ctx->ticket, 1, st);
     nnhip::launch_block_tables(st, B, cached, added, lbs, max_blocks, tables, held, num_blocks,
                                free_list, free_count, T, row_start, lens, pos, slots, status,
                                ctx->ticket.p);
@@ -117,9 +121,17 @@ int nnhip_attention_paged_q8(nnhip_ctx *ctx, const float *q, int T, const int8_t
     REQ(ctx && tables && row_start && lens && T >= 0 && ((q && out) || T == 0),
         "nnhip_attention_paged_q8: NULL argument or negative T");
     if (T == 0) return;
+    REQ((int64_t)T * H <= INT32_MAX, "nnhip_attention_paged_q8: more than 2^31 - 1 rows of heads");
     set_device(ctx);
-    nnhip::launch_attention_paged(ctx->c.stream, q, T, codes, scales, p, tables, max_blocks,
-                                  row_start, lens, B, H, out);
+    hipStream_t st = ctx->c.stream;
+    if (!ctx->paged_tickets.p) zeroed(ctx->paged_tickets, nnhip::attention_paged_tickets(), st);
+    const size_t need = (size_t)nnhip::attention_paged_part_elems(D);
+    if (need > ctx->paged_part.n) {
+      NNHIP_CHECK(hipStreamSynchronize(st));   // earlier calls may read it
+      ctx->paged_part.ensure(need);
+    }
+    nnhip::launch_attention_paged(st, q, T, codes, scales, p, tables, max_blocks, row_start, lens, B,
+                                  H, out, ctx->paged_part.p, ctx->paged_tickets.p);
   });
 }
 
