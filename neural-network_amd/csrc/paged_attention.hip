@@ -111,7 +111,7 @@ struct AttnArgs {
 
 // 16 columns of a request: column c is row first + c / G, head hk * G + c % G.
 struct Columns {
-  int b, first, n, base;         // base: the tile's first column
+  int first, n, base;            // the request's rows, the tile's first column
   int64_t len;
 };
 
@@ -129,12 +129,12 @@ __device__ inline Query<D> load_query(const AttnArgs &a, const Columns &c, int h
   const int col = c.base + (lane & 15), g = lane >> 4;
   const bool live = col < c.n * a.G;
   const int row = live ? col / a.G : 0, h = hk * a.G + (live ? col % a.G : 0);
-  const float *src = a.q + ((int64_t)(c.first + row) * a.H + h) * D + g * (D / 4);
+  const float *src = a.q + ((int64_t)(c.first + row) * a.H + h) * D + g * (D == 32 ? 8 : 16);
   float x[D / 4];
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    const float4 v = *reinterpret_cast<const float4 *>(src + 4 * i);
+    const float4 v = *reinterpret_cast<const float4 *>(src + 64 * (i / 4) + 4 * (i % 4));
     x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
   }
 #pragma unroll
@@ -235,26 +235,32 @@ __device__ inline void softmax_tile(State<D> &s, const float4_t (&acc)[4], float
 // S^T = K Q^T and O^T = V^T P^T: the codes are the left operand, as they lie in
 // memory, and the weights that the first product leaves in a lane are what the
 // second one wants there.  Lane (r = lane & 15, g = lane >> 4): the left operand of
-// score product t holds, in row r, token 16 (r >> 2) + 4 t + (r & 3), dims
-// g D/4 .. (g + 1) D/4 - 1 (the order of the dims is free), so that lane
-// (column, g) gets the scores of tokens 16 g + 4 t + i, all of one block; the left
-// operand of the products with v holds dim 16 d + r, the 16 tokens of block g.
+// score product t holds, in row r, token 16 (r >> 2) + 4 t + (r & 3), dims 16 g ..
+// 16 g + 15 of each 64 (the order of the dims is free: four lanes load 64
+// neighbouring bytes), so that lane (column, g) gets the scores of tokens 16 g +
+// 4 t + i, all of one block; the left operand of the products with v holds dim
+// 16 d + r, the 16 tokens of block g.
 constexpr int kSplitWaves = 4, kSplitThreads = kWave * kSplitWaves;
-constexpr int kSplitUnits = 1024;   // units that a launch is split into, if it has the tiles
+constexpr int kSplitUnits = 512;    // units that a launch is split into, if it has the tiles
 constexpr int kSplitMin = 4;        // least tiles of a split
 
 struct Part {                        // a request's share of the work
-  int tiles, groups, splits;         // key tiles, tiles of columns, units a group
+  int first, n, len;                 // its rows, its tokens
+  int tiles, groups;                 // tiles of keys, tiles of columns
 };
-__device__ inline Part part_of(const AttnArgs &a, int b, int64_t chunk) {
+__device__ inline Part part_of(const AttnArgs &a, int b) {
   const RowRange r = request_rows(a.row_start, b, a.T);
-  const int n = r.last - r.first;
-  if (n == 0) return Part{0, 0, 0};
-  const int tiles =
-      (int)((request_len(a.lens[b], a.max_blocks, a.p.lbs) + kKeys - 1) / kKeys);
-  const int groups = (int)(((int64_t)n * a.G + kCols - 1) / kCols);
-  const int splits = chunk ? max(1, (int)((tiles + chunk - 1) / chunk)) : 0;
-  return Part{tiles, groups, splits};
+  const int len = (int)request_len(a.lens[b], a.max_blocks, a.p.lbs);
+  Part p{r.first, r.last - r.first, len, 0, 0};
+  if (p.n) {
+    p.tiles = (int)(((int64_t)len + kKeys - 1) / kKeys);
+    p.groups = (int)(((int64_t)p.n * a.G + kCols - 1) / kCols);
+  }
+  return p;
+}
+// Units of one group and kv head.
+__device__ inline int splits_of(const Part &p, int64_t chunk) {
+  return max(1, (int)((p.tiles + chunk - 1) / chunk));
 }
 
 // Sums over the 256 threads before and including `tid`; the last entry is all.
@@ -277,7 +283,7 @@ __device__ inline void load_k(const AttnArgs &a, const Sub &s, int hk, int lane,
                               uint32_t (&r)[4][D / 16]) {
   const int m = lane & 15, g = lane >> 4;
   const int8_t *src = a.codes + head_offset(a.p, s.blk, 0, hk) +
-                      (int64_t)(s.off + (m & 3)) * D + g * (D / 4);
+                      (int64_t)(s.off + (m & 3)) * D + g * (D == 32 ? 8 : 16);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if constexpr (D == 32) {
@@ -286,7 +292,7 @@ __device__ inline void load_k(const AttnArgs &a, const Sub &s, int hk, int lane,
     } else {
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(src + 4 * t * D + 16 * i);
+        const uint4 v = *reinterpret_cast<const uint4 *>(src + 4 * t * D + 64 * i);
         r[t][4 * i] = v.x; r[t][4 * i + 1] = v.y; r[t][4 * i + 2] = v.z; r[t][4 * i + 3] = v.w;
       }
     }
@@ -305,56 +311,135 @@ __device__ inline void load_v(const AttnArgs &a, const Sub &s, int hk, int lane,
   }
 }
 
+// Joins the shares of a group's units, `step` floats apart: a wave at a time takes
+// a column's exponents (a lane a unit), then the threads the sums, eight units'
+// loads in flight.  lds: at least 16 x 64 floats.
+template <int D>
+__device__ inline void join(const AttnArgs &a, const Columns &c, int hk, int cols, const float *src,
+                            int64_t step, int splits, float *lds, float *s_m, float *s_l) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int col = wave; col < cols; col += kSplitWaves) {
+    float M = -INFINITY, L = 0.f;
+    for (int s = lane; s < splits; s += kWave) M = fmaxf(M, src[s * step + col * (D + 2) + D]);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
+    for (int s = lane; s < splits; s += kWave) {
+      const float *p = src + s * step + col * (D + 2) + D;
+      L = fmaf(p[1], share(p[0], M), L);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, kWave);
+    if (lane == 0) {
+      s_m[col] = M;
+      s_l[col] = L == 0.f ? 1.f : L;
+    }
+  }
+  __syncthreads();
+  constexpr int kTasks = kCols * D / 4, kPer = (kTasks + kSplitThreads - 1) / kSplitThreads;
+  const int tasks = cols * (D / 4);
+  float4_t o[kPer] = {};
+  for (int s0 = 0; s0 < splits; s0 += kWave) {
+    const int n = min(kWave, splits - s0);
+    for (int i = tid; i < cols * kWave; i += kSplitThreads) {
+      const int col = i / kWave, s = i % kWave;
+      lds[i] = s < n ? share(src[(s0 + s) * step + col * (D + 2) + D], s_m[col]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = tid + k * kSplitThreads, col = i / (D / 4);
+      if (i >= tasks) continue;
+      const float *at = src + s0 * step + col * (D + 2) + 4 * (i % (D / 4));
+      for (int s = 0; s < n; s += 8) {
+        float2 x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float *q = at + min(s + e, n - 1) * step;
+          x[e] = *reinterpret_cast<const float2 *>(q);
+          y[e] = *reinterpret_cast<const float2 *>(q + 2);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (s + e < n) {
+            const float f = lds[col * kWave + s + e];
+            o[k][0] = fmaf(x[e].x, f, o[k][0]);
+            o[k][1] = fmaf(x[e].y, f, o[k][1]);
+            o[k][2] = fmaf(y[e].x, f, o[k][2]);
+            o[k][3] = fmaf(y[e].y, f, o[k][3]);
+          }
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int i = tid + k * kSplitThreads, col = i / (D / 4), x = c.base + col;
+    if (i < tasks)
+      *reinterpret_cast<float4_t *>(
+          a.out + ((int64_t)(c.first + x / a.G) * a.H + hk * a.G + x % a.G) * D +
+          4 * (i % (D / 4))) = o[k] / s_l[col];
+  }
+}
+
 __device__ inline void put2(float *p, float x, float y) {
   const uint64_t bits = ((uint64_t)__float_as_uint(y) << 32) | __float_as_uint(x);
   __hip_atomic_store(reinterpret_cast<uint64_t *>(p), bits, __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ inline float2 get2(const float *p) {
-  const uint64_t bits = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED,
-                                          __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__uint_as_float((uint32_t)bits), __uint_as_float((uint32_t)(bits >> 32)));
-}
-
 template <int D>
 __global__ __launch_bounds__(kSplitThreads, 2) void attn_paged_split_kernel(
     AttnArgs a, float *__restrict__ part, unsigned *__restrict__ tickets) {
   constexpr int kOut = D + 4;        // a column's sums in LDS
   __shared__ float s_o[kSplitWaves][kCols][kOut];
   __shared__ float s_m[kSplitWaves][kCols], s_l[kSplitWaves][kCols], s_e[kSplitWaves][kCols];
-  __shared__ int s_items[kSplitThreads], s_pick[8], s_sum[kSplitWaves];
-  __shared__ int64_t s_tiles[kSplitWaves];
+  __shared__ int s_pick[12], s_sum[kSplitWaves];
+  __shared__ int64_t s_tiles[2][kSplitWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int Hkv = a.p.Hkv, per = (a.B + kSplitThreads - 1) / kSplitThreads;
   const int b0 = tid * per, b1 = min(a.B, b0 + per);
-  int64_t work = 0;
+  // up to 256 requests: one a thread, read once
+  const Part only = b0 < b1 ? part_of(a, b0) : Part{0, 0, 0, 0, 0};
+  auto part_at = [&](int b) { return b == b0 ? only : part_of(a, b); };
+  int64_t work = 0, groups = 0;
   for (int b = b0; b < b1; ++b) {
-    const Part p = part_of(a, b, 0);
+    const Part p = part_at(b);
     work += (int64_t)p.tiles * p.groups;
+    groups += p.groups;
   }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) work += __shfl_xor(work, o, kWave);
-  if (lane == 0) s_tiles[wave] = work;
+  for (int o = 32; o; o >>= 1) {
+    work += __shfl_xor(work, o, kWave);
+    groups += __shfl_xor(groups, o, kWave);
+  }
+  if (lane == 0) {
+    s_tiles[0][wave] = work;
+    s_tiles[1][wave] = groups;
+  }
   __syncthreads();
-  work = 0;
-  for (int w = 0; w < kSplitWaves; ++w) work += s_tiles[w];
-  const int64_t chunk =
-      max((int64_t)kSplitMin, (work * Hkv + kSplitUnits - 1) / kSplitUnits);
+  work = groups = 0;
+  for (int w = 0; w < kSplitWaves; ++w) {
+    work += s_tiles[0][w];
+    groups += s_tiles[1][w];
+  }
+  // a group of tiles / chunk + 1 units at most: all units run at once
+  const int64_t room = max((int64_t)kSplitUnits / 4, kSplitUnits - groups * Hkv);
+  const int64_t chunk = max((int64_t)kSplitMin, (work * Hkv + room - 1) / room);
   int mine = 0, shared = 0, sgroups = 0;     // units of a kv head; those and groups that are split
   for (int b = b0; b < b1; ++b) {
-    const Part p = part_of(a, b, chunk);
-    mine += p.groups * p.splits;
-    if (p.splits > 1) {
-      shared += p.groups * p.splits;
+    const Part p = part_at(b);
+    const int splits = splits_of(p, chunk);
+    mine += p.groups * splits;
+    if (splits > 1) {
+      shared += p.groups * splits;
       sgroups += p.groups;
     }
   }
   const int upto = block_scan(mine, tid, s_sum);
   const int sat = block_scan(shared, tid, s_sum) - shared;
   const int gat = block_scan(sgroups, tid, s_sum) - sgroups;
-  s_items[tid] = upto;
+  if (tid == kSplitThreads - 1) s_pick[11] = upto;
   __syncthreads();
-  const int units = s_items[kSplitThreads - 1] * Hkv;
+  const int units = s_pick[11] * Hkv;
 
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int item = u / Hkv, hk = u % Hkv;
@@ -362,21 +447,24 @@ __global__ __launch_bounds__(kSplitThreads, 2) void attn_paged_split_kernel(
     if (item < upto && item >= upto - mine) {
       int at = upto - mine, sb = sat, gb = gat;
       for (int b = b0; b < b1; ++b) {
-        const Part p = part_of(a, b, chunk);
-        const int k = p.groups * p.splits;
+        const Part p = part_at(b);
+        const int splits = splits_of(p, chunk), k = p.groups * splits;
         if (item < at + k) {
-          const int x = item - at, grp = x / p.splits;
+          const int x = item - at, grp = x / splits;
           s_pick[0] = b;
           s_pick[1] = grp;
-          s_pick[2] = x % p.splits;
-          s_pick[3] = p.splits;
+          s_pick[2] = x % splits;
+          s_pick[3] = splits;
           s_pick[4] = p.tiles;
           s_pick[5] = sb + x;
           s_pick[6] = gb + grp;
+          s_pick[8] = p.first;
+          s_pick[9] = p.n;
+          s_pick[10] = p.len;
           break;
         }
         at += k;
-        if (p.splits > 1) {
+        if (splits > 1) {
           sb += k;
           gb += p.groups;
         }
@@ -385,10 +473,7 @@ __global__ __launch_bounds__(kSplitThreads, 2) void attn_paged_split_kernel(
     __syncthreads();
     const int b = s_pick[0], grp = s_pick[1], split = s_pick[2], splits = s_pick[3];
     const int tiles = s_pick[4], slot = s_pick[5] * Hkv + hk, group = s_pick[6] * Hkv + hk;
-    const RowRange rr = request_rows(a.row_start, b, a.T);
-    const Columns c{b, rr.first, rr.last - rr.first, grp * kCols,
-                    request_len(a.lens[b], a.max_blocks, a.p.lbs)};
-    const Query<D> q = load_query<D>(a, c, hk, lane);
+    const Columns c{s_pick[8], s_pick[9], grp * kCols, s_pick[10]};
     // key tiles of the unit: of the last row's tokens at most
     const int cols = min(kCols, c.n * a.G - c.base);
     const int64_t most = max((int64_t)0, c.len - c.n + (c.base + cols - 1) / a.G + 1);
@@ -407,6 +492,7 @@ __global__ __launch_bounds__(kSplitThreads, 2) void attn_paged_split_kernel(
       float ksc = a.scales[scale_offset(a.p, vs.blk, 0, hk)];
       float vsc = a.scales[scale_offset(a.p, vs.blk, 1, hk)];
       load_v<D>(a, vs, hk, lane, vr);
+      const Query<D> q = load_query<D>(a, c, hk, lane);
       bool bad = vs.bad;
       for (; t < t1; t += kSplitWaves) {
         const int64_t next = (int64_t)(t + kSplitWaves) * kKeys;
@@ -497,28 +583,10 @@ __global__ __launch_bounds__(kSplitThreads, 2) void attn_paged_split_kernel(
       if (tid == 0) s_pick[7] = atomicAdd(tickets + group, 1u) == (unsigned)splits - 1;
       __syncthreads();
       if (s_pick[7]) {
-        // units of a group are Hkv slots apart
-        const float *src = mine_part - (int64_t)split * Hkv * kCols * (D + 2);
-        const int64_t step = (int64_t)Hkv * kCols * (D + 2);
-        for (int i = tid; i < cols * (D / 4); i += kSplitThreads) {
-          const int cc = i / (D / 4), d4 = i % (D / 4);
-          const float *at = src + cc * (D + 2);
-          float M = -INFINITY, L = 0.f;
-          float4_t o = {};
-          for (int s = 0; s < splits; ++s) M = fmaxf(M, get2(at + s * step + D).x);
-          for (int s = 0; s < splits; ++s) {
-            const float2 ml = get2(at + s * step + D);
-            const float2 x = get2(at + s * step + 4 * d4), y = get2(at + s * step + 4 * d4 + 2);
-            const float f = share(ml.x, M);
-            L = fmaf(ml.y, f, L);
-            o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]);
-            o[2] = fmaf(y.x, f, o[2]); o[3] = fmaf(y.y, f, o[3]);
-          }
-          if (L == 0.f) L = 1.f;
-          const int x = c.base + cc;
-          *reinterpret_cast<float4_t *>(
-              a.out + ((int64_t)(c.first + x / a.G) * a.H + hk * a.G + x % a.G) * D + 4 * d4) = o / L;
-        }
+        // what the others stored is read past this die's caches
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        join<D>(a, c, hk, cols, mine_part - (int64_t)split * Hkv * kCols * (D + 2),
+                (int64_t)Hkv * kCols * (D + 2), splits, &s_o[0][0][0], s_m[0], s_l[0]);
         if (tid == 0) atomicExch(tickets + group, 0u);
       }
     }
@@ -528,10 +596,10 @@ __global__ __launch_bounds__(kSplitThreads, 2) void attn_paged_split_kernel(
 
 template <int D>
 void launch_split(hipStream_t st, const AttnArgs &a, float *part, unsigned *tickets) {
-  // as many workgroups as there can be units, up to four a CU; the rest in turn
+  // as many workgroups as there can be units, up to two a CU; the rest in turn
   const int64_t bound = (int64_t)kSplitUnits +
       (((int64_t)a.T * a.G + kCols - 1) / kCols + std::min(a.B, a.T)) * a.p.Hkv;
-  const int grid = (int)std::min<int64_t>(bound, 1024);
+  const int grid = (int)std::min<int64_t>(bound, kSplitUnits);
   hipLaunchKernelGGL(attn_paged_split_kernel<D>, dim3(grid), dim3(kSplitThreads), 0, st, a, part,
                      tickets);
 }
