@@ -389,7 +389,7 @@ int nnhip_spec_accept(nnhip_ctx *ctx, const float *tlogits,
  * scale for each block and head where KVCache(true) has one for each row.
  *
  * Pool: num_blocks blocks of block_size tokens (16, 32, 64 or 128; at most
- * 2^31 - 1 slots in all).
+ * 2^31 - 1 slots in all; a table row names at most 2^30 tokens).
  *   codes  [num_blocks][2][Hkv][block_size * D] int8, aligned to 16 bytes:
  *          k (index 0) as [block_size][D], v (index 1) as [D][block_size]
  *   scales [num_blocks][2][Hkv] fp32, not negative; a cached value is code *

@@ -64,8 +64,8 @@ int nnhip_block_tables(nnhip_ctx *ctx, int B, const int32_t *cached, const int32
     const int lbs = block_shift(block_size, what);
     REQ(num_blocks > 0 && (int64_t)num_blocks * block_size <= INT32_MAX,
         "nnhip_block_tables: num_blocks must be positive, with at most 2^31 - 1 token slots");
-    REQ(max_blocks > 0 && (int64_t)max_blocks * block_size <= INT32_MAX,
-        "nnhip_block_tables: max_blocks must be positive, with at most 2^31 - 1 tokens");
+    REQ(max_blocks > 0 && (int64_t)max_blocks * block_size <= 1 << 30,
+        "nnhip_block_tables: max_blocks must be positive, with at most 2^30 tokens a request");
     REQ(T >= 0, "nnhip_block_tables: T is negative");
     REQ(ctx && cached && added && tables && held && free_list && free_count && row_start && lens &&
             status && ((pos && slots) || T == 0),
@@ -114,8 +114,8 @@ int nnhip_attention_paged_q8(nnhip_ctx *ctx, const float *q, int T, const int8_t
     const nnhip::PagedPool p = pool_of(block_size, num_blocks, Hkv, D, codes, scales, what);
     check_heads(H, Hkv, what);
     REQ(B > 0 && B <= nnhip::kMaxRequests, "nnhip_attention_paged_q8: B must be in [1, 4096]");
-    REQ(max_blocks > 0 && (int64_t)max_blocks * block_size <= INT32_MAX,
-        "nnhip_attention_paged_q8: max_blocks must be positive, with at most 2^31 - 1 tokens");
+    REQ(max_blocks > 0 && (int64_t)max_blocks * block_size <= 1 << 30,
+        "nnhip_attention_paged_q8: max_blocks must be positive, with at most 2^30 tokens a request");
     REQ(aligned(q, 16) && aligned(out, 16),
         "nnhip_attention_paged_q8: q and out must be aligned to 16 bytes");
     REQ(ctx && tables && row_start && lens && T >= 0 && ((q && out) || T == 0),

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 
 namespace nnhip {
 
@@ -33,6 +34,14 @@ constexpr int kNone = -(1 << 20);  // E before the first contribution
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+
+// threadIdx.x for one stretch of code: what is formed from it is formed there, and
+// not kept in registers over the loops around.
+__device__ inline int thread_here() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
 
 __device__ inline half2_t as_half2(uint32_t x) { return __builtin_bit_cast(half2_t, x); }
 __device__ inline uint32_t as_u32(half2_t x) { return __builtin_bit_cast(uint32_t, x); }
@@ -70,20 +79,6 @@ __device__ inline float sum_groups(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Where the codes and scales of 16 tokens lie: their block, and the first one's
-// place in it.  Tokens behind the request's last are read from block 0 (and
-// masked), tokens of a block outside the pool too, with `bad`.
-struct Sub { int blk, off; bool bad; };
-__device__ inline Sub sub_of(const int32_t *table, int64_t tok, int64_t len, const PagedPool &p) {
-  Sub s{0, (int)tok & (p.bs - 1), false};
-  if (tok < len) {
-    const int blk = table[tok >> p.lbs];
-    s.bad = !block_ok(blk, p.blocks);
-    s.blk = s.bad ? 0 : blk;
-  }
-  return s;
-}
-
 // A scale as it is used: NaN unless it is a number >= 0; 0 below 2^-126, where a
 // logarithm and the products lose it.
 __device__ inline float scale_ok(float s, bool bad) {
@@ -107,34 +102,446 @@ struct AttnArgs {
   const int32_t *row_start, *lens;
   int B, H, G;                   // G: heads of q for one of k and v
   float *out;
+  bool tall;                     // requests of many columns run in the tall kernel
 };
 
-// 16 columns of a request: column c is row first + c / G, head hk * G + c % G.
+// Blocks and scales of 16 key tiles, `step` tiles apart, a lane for each of a tile's
+// four times 16 tokens: read once and passed between the lanes, so that no tile's
+// loads wait for the table.  Tokens behind the request's last (len > 0) take its
+// block, and are masked; a block outside the pool is read as block 0, with scales
+// that make what sees it NaN, as a scale that is no number does.
+constexpr int kHeld = 16;
+struct Held { int blk; float ks, vs, lvs; };   // lvs: log2(vs)
+__device__ inline Held held_tiles(const AttnArgs &a, const int32_t *table, int tile, int step, int len,
+                                  int hk) {
+  const int lane = threadIdx.x & 63;
+  const int tok = (tile + (lane >> 2) * step) * kKeys + 16 * (lane & 3);
+  const int blk = table[min(tok, len - 1) >> a.p.lbs];
+  const bool bad = !block_ok(blk, a.p.blocks);
+  Held r;
+  r.blk = bad ? 0 : blk;
+  r.ks = scale_ok(a.scales[scale_offset(a.p, r.blk, 0, hk)], bad);
+  r.vs = scale_ok(a.scales[scale_offset(a.p, r.blk, 1, hk)], bad);
+  if (r.vs != r.vs) r.ks = r.vs;
+  r.lvs = __builtin_amdgcn_logf(r.vs);
+  return r;
+}
+
+// Columns of a request: column c is row first + c / G, head hk * G + c % G.
 struct Columns {
-  int first, n, base;            // the request's rows, the tile's first column
-  int64_t len;
+  int first, n, base;            // the request's rows, the unit's first column
+  int len;
+  const int32_t *table;
+};
+__device__ inline float *out_row(const AttnArgs &a, const Columns &c, int hk, int col, int D) {
+  const int x = c.base + col;
+  return a.out + ((int64_t)(c.first + x / a.G) * a.H + hk * a.G + x % a.G) * D;
+}
+
+__device__ inline void put2(float *p, float x, float y) {
+  const uint64_t bits = ((uint64_t)__float_as_uint(y) << 32) | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), bits, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The power of two that takes a row's largest element to [2^13, 2^14).
+__device__ inline int query_shift(float top) {
+  return min(13 + 127 - (int)((__float_as_uint(top) >> 23) & 255), 120);
+}
+// Two weights as halves and what these leave.
+__device__ inline void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.f, x),
+                                                               fmaf((float)h[1], -1.f, y)));
+}
+
+// ---------------------------------------------------------------------------
+// Units.
+//
+// A unit is a tile of columns of one request and kv head over a range of `chunk`
+// key tiles: 128 columns where a request has at least kTallFrom of them
+// (attn_paged_tall_kernel), else 16 (attn_paged_short_kernel).  The lengths are on
+// the device, so every workgroup forms the sums over the requests itself and takes
+// its units from them; the ranges are chosen so that the units of a launch fill the
+// chip, whatever the lengths are.  Where a group of columns has several ranges, each
+// unit leaves its state in the scratch, and the last to arrive (a counter a group,
+// left zero) joins them.
+constexpr int kShortWaves = 4, kTallWaves = 8, kMostWaves = 8;
+constexpr int kTallCols = kCols * kTallWaves, kTallFrom = kPagedTallFrom;
+constexpr int kSlots = 512;              // workgroups that run at once: two a CU
+constexpr int kShortRoom = kSlots / 4;   // least slots that are shared out by tiles
+constexpr int kShortMin = 8, kTallMin = 4;   // least tiles of a unit of several
+
+struct Part {                            // a request's share of the work
+  int first, n, len;                     // its rows, its tokens
+  int groups;                            // tiles of columns
+};
+// TALL: requests of many columns, else the others (all, if no tall kernel runs).
+template <bool TALL>
+__device__ inline Part part_of(const AttnArgs &a, int b) {
+  const RowRange r = request_rows(a.row_start, b, a.T);
+  const int len = (int)request_len(a.lens[b], a.max_blocks, a.p.lbs);
+  Part p{r.first, r.last - r.first, len, 0};
+  const int64_t cols = (int64_t)p.n * a.G;
+  const bool tall = a.tall && cols >= kTallFrom;
+  constexpr int kWide = TALL ? kTallCols : kCols;
+  if (tall == TALL) p.groups = (int)((cols + kWide - 1) / kWide);
+  return p;
+}
+__device__ inline int tiles_of(const Part &p) { return (p.len + kKeys - 1) / kKeys; }
+// Tokens that column x of a request sees.
+__device__ inline int seen_by(int len, int n, int x, int G) { return max(0, len - n + x / G + 1); }
+
+// The ranges of a request.  Short: every group has all of them.  Tall: a group has
+// those that its last row sees something of, so range s has groups first_group(s)
+// and on: the groups of a row i with len - n + i >= s chunk 64.
+template <bool TALL>
+struct Ranges {
+  int count;                             // of the last group
+  int shared;                            // first group that has several
+  int chunk, groups;
+  int64_t past, G;
+
+  __device__ Ranges(const Part &p, int chunk_, int G_)
+      : chunk(chunk_), groups(p.groups), past((int64_t)p.len - p.n), G(G_) {
+    count = max(1, (tiles_of(p) + chunk - 1) / chunk);
+    shared = count > 1 ? first_group(1) : groups;
+  }
+  __device__ int first_group(int s) const {
+    if (!TALL || s == 0) return 0;
+    const int64_t row = max((int64_t)0, (int64_t)s * chunk * kKeys - past);
+    return (int)min((int64_t)groups, row * G / kTallCols);
+  }
+  __device__ int units() const {
+    if (!TALL) return groups * count;
+    int u = 0;
+    for (int s = 0; s < count; ++s) u += groups - first_group(s);
+    return u;
+  }
+  // units that share their group
+  __device__ int shares() const { return shared < groups ? units() - shared : 0; }
+  // ranges of group g
+  __device__ int of_group(int g) const {
+    if (!TALL) return count;
+    int s = 1;
+    while (s < count && first_group(s) <= g) ++s;
+    return s;
+  }
+  // place of (group g, range s) among the request's shares, range by range
+  __device__ int place(int g, int s) const {
+    int at = 0;
+    for (int i = 0; i < s; ++i) at += groups - max(shared, first_group(i));
+    return at + g - max(shared, first_group(s));
+  }
 };
 
-// The q of a lane's column, and what its scores are multiplied by.
+// Sums over a wave, up to and including each lane.
+__device__ inline int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+
+struct Pick {                            // a unit
+  int b, group, range, ranges, first, n, len, groups;
+  int slot, ticket;                      // the request's first, for kv head 0
+};
+constexpr int kPickWords = 10;
+constexpr int kAhead = 8;                // units that a workgroup looks up at a time
+
+struct PlanMem {
+  int pick[kAhead][kPickWords];
+  float work[kMostWaves];
+  int sum[kMostWaves][3];
+  int chunk, last;
+};
+
+// Place of the k-th unit of a workgroup in the order in which units are dealt out:
+// rounds of all workgroups, every other one backwards, so that who had a long unit
+// gets a short one next.
+__device__ inline int64_t place_of(int64_t k) {
+  const int64_t r = k * gridDim.x;
+  return r + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+// The workgroup's units k0 .. k0 + kAhead - 1; returns the number of all units.
+template <bool TALL, int WAVES>
+__device__ inline int plan_units(const AttnArgs &a, int64_t k0, PlanMem &s) {
+  constexpr int kThreads = WAVES * kWave;
+  const int tid = thread_here(), lane = tid & 63, wave = tid >> 6, Hkv = a.p.Hkv;
+  // a few consecutive requests a thread (one, up to as many as there are threads)
+  const int per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(a.B, b0 + per);
+  const Part only = b0 < b1 ? part_of<TALL>(a, b0) : Part{0, 0, 0, 0};
+  auto part_at = [&](int b) { return b == b0 ? only : part_of<TALL>(a, b); };
+  // tiles of all groups, from above: fp32 sums are off by 2^-14 at most
+  float work = 0.f;
+  int groups = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Part p = part_at(b);
+    const float g = (float)p.groups;
+    work += TALL ? g * (max(0, p.len - p.n) + 1) / kKeys + g * (g + 1.f) * kCols * kTallWaves / 2 /
+                           (kKeys * (float)a.G) + g
+                 : g * (float)tiles_of(p);
+    groups += p.groups;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) work += __shfl_xor(work, o, kWave);
+  groups = wave_scan(groups);
+  if (lane == 63) {
+    s.work[wave] = work;
+    s.sum[wave][0] = groups;
+  }
+  __syncthreads();
+  work = 0.f;
+  groups = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    work += s.work[w];
+    groups += s.sum[w][0];
+  }
+  __syncthreads();
+  // Short: work / chunk + groups units, all at once.  Tall: no unit longer than a
+  // slot's part of the work, for the rows of a prompt see more and more tokens.
+  const int room = TALL ? kSlots
+                        : groups < kSlots ? max(kShortRoom, kSlots - groups * Hkv) : kShortRoom;
+  const float target = work * (1.f + 1.f / 8192) * Hkv / room;
+  const int chunk = max(TALL ? kTallMin : kShortMin, (int)fminf(target, 1e6f) + 1);
+  int mine = 0, shares = 0, shared = 0;      // units, those that share a group, such groups
+  for (int b = b0; b < b1; ++b) {
+    const Part p = part_at(b);
+    const Ranges<TALL> r(p, chunk, a.G);
+    mine += r.units();
+    shares += r.shares();
+    shared += p.groups - r.shared;
+  }
+  int upto = wave_scan(mine), sat = wave_scan(shares), gat = wave_scan(shared);
+  if (lane == 63) {
+    s.sum[wave][0] = upto;
+    s.sum[wave][1] = sat;
+    s.sum[wave][2] = gat;
+  }
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    all += s.sum[w][0];
+    if (w < wave) {
+      upto += s.sum[w][0];
+      sat += s.sum[w][1];
+      gat += s.sum[w][2];
+    }
+  }
+  sat -= shares;
+  gat -= shared;
+  for (int k = 0; k < kAhead; ++k) {
+    const int64_t at = place_of(k0 + k);
+    if (at >= (int64_t)all * Hkv) continue;
+    // the thread whose requests hold the unit writes it down
+    int x = (int)((uint32_t)at / Hkv) - (upto - mine);
+    if (x < 0 || x >= mine) continue;
+    int slot = sat, ticket = gat;
+    for (int b = b0; b < b1; ++b) {
+      const Part p = part_at(b);
+      const Ranges<TALL> r(p, chunk, a.G);
+      const int units = r.units();
+      if (x >= units) {
+        x -= units;
+        slot += r.shares();
+        ticket += p.groups - r.shared;
+        continue;
+      }
+      // range by range, a prompt's last rows, which see the most, first; short
+      // groups one by one
+      int g, range = 0;
+      if (TALL) {
+        while (x >= p.groups - r.first_group(range)) x -= p.groups - r.first_group(range++);
+        g = p.groups - 1 - x;
+      } else {
+        g = x / r.count;
+        range = x % r.count;
+      }
+      int *out = s.pick[k];
+      out[0] = b;
+      out[1] = g;
+      out[2] = range;
+      out[3] = r.of_group(g);
+      out[4] = p.first;
+      out[5] = p.n;
+      out[6] = p.len;
+      out[7] = p.groups;
+      out[8] = slot;
+      out[9] = ticket + g - r.shared;
+      break;
+    }
+  }
+  if (tid == 0) s.chunk = chunk;
+  __syncthreads();
+  return all * Hkv;
+}
+
+// A group's units have left their shares and arrive here; whether this is the
+// last of them, which joins.
+__device__ inline bool last_of(unsigned *ticket, int ranges, int *s_last) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) *s_last = atomicAdd(ticket, 1u) == (unsigned)ranges - 1;
+  __syncthreads();
+  if (!*s_last) return false;
+  if (threadIdx.x == 0) atomicExch(ticket, 0u);
+  // what the others stored is read past this die's caches
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  return true;
+}
+
+// Joins the shares of a group's units: a column's exponents and weights first, a
+// lane a unit, then the sums, a thread for four of a column, eight units' loads in
+// flight.  at(s): the unit's share.
+struct JoinMem { float w[kCols][kWave], m[kCols], l[kCols]; };
+template <int D, int WAVES, typename At>
+__device__ inline void join(const AttnArgs &a, const Columns &c, int hk, int cols, int ranges,
+                            JoinMem &s, At at) {
+  constexpr int kThreads = WAVES * kWave;
+  const int tid = thread_here(), lane = tid & 63, wave = tid >> 6;
+  for (int col0 = 0; col0 < cols; col0 += kCols) {
+    const int here = min(kCols, cols - col0);
+    for (int col = wave; col < here; col += WAVES) {
+      float M = -INFINITY, L = 0.f;
+      for (int r = lane; r < ranges; r += kWave) M = fmaxf(M, at(r)[(col0 + col) * (D + 2) + D]);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
+      for (int r = lane; r < ranges; r += kWave) {
+        const float *p = at(r) + (col0 + col) * (D + 2) + D;
+        L = fmaf(p[1], share(p[0], M), L);
+      }
+#pragma unroll
+      for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, kWave);
+      if (lane == 0) {
+        s.m[col] = M;
+        s.l[col] = L == 0.f ? 1.f : L;       // no token is seen: the sums are 0
+      }
+    }
+    __syncthreads();
+    constexpr int kPer = (kCols * D / 4 + kThreads - 1) / kThreads;
+    float4_t o[kPer] = {};
+    for (int r0 = 0; r0 < ranges; r0 += kWave) {
+      const int n = min(kWave, ranges - r0);
+      for (int i = tid; i < here * kWave; i += kThreads) {
+        const int col = i / kWave, r = i % kWave;
+        s.w[col][r] = r < n ? share(at(r0 + r)[(col0 + col) * (D + 2) + D], s.m[col]) : 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int i = tid + k * kThreads, col = i / (D / 4);
+        if (col >= here) continue;
+        const int off = (col0 + col) * (D + 2) + 4 * (i % (D / 4));
+        for (int r = 0; r < n; r += 8) {
+          float2 x[8], y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float *q = at(r0 + min(r + e, n - 1)) + off;
+            x[e] = *reinterpret_cast<const float2 *>(q);
+            y[e] = *reinterpret_cast<const float2 *>(q + 2);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (r + e < n) {
+              const float f = s.w[col][r + e];
+              o[k][0] = fmaf(x[e].x, f, o[k][0]);
+              o[k][1] = fmaf(x[e].y, f, o[k][1]);
+              o[k][2] = fmaf(y[e].x, f, o[k][2]);
+              o[k][3] = fmaf(y[e].y, f, o[k][3]);
+            }
+        }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = tid + k * kThreads, col = i / (D / 4);
+      if (col < here)
+        *reinterpret_cast<float4_t *>(out_row(a, c, hk, col0 + col, D) + 4 * (i % (D / 4))) =
+            o[k] / s.l[col];
+    }
+    __syncthreads();
+  }
+}
+// The same for a few units, nothing shared between the threads.
+constexpr int kFew = 8;
+template <int D, int WAVES, typename At>
+__device__ inline void join_few(const AttnArgs &a, const Columns &c, int hk, int cols, int ranges,
+                                At at) {
+  for (int i = thread_here(); i < cols * (D / 4); i += WAVES * kWave) {
+    const int col = i / (D / 4), d4 = i % (D / 4);
+    float2 ml[kFew], x[kFew], y[kFew];
+#pragma unroll
+    for (int r = 0; r < kFew; ++r) {
+      const float *q = at(min(r, ranges - 1)) + col * (D + 2);
+      ml[r] = *reinterpret_cast<const float2 *>(q + D);
+      x[r] = *reinterpret_cast<const float2 *>(q + 4 * d4);
+      y[r] = *reinterpret_cast<const float2 *>(q + 4 * d4 + 2);
+    }
+    float M = ml[0].x, L = 0.f;
+#pragma unroll
+    for (int r = 1; r < kFew; ++r) M = fmaxf(M, ml[r].x);
+    float4_t o = {};
+#pragma unroll
+    for (int r = 0; r < kFew; ++r)
+      if (r < ranges) {
+        const float f = share(ml[r].x, M);
+        L = fmaf(ml[r].y, f, L);
+        o[0] = fmaf(x[r].x, f, o[0]);
+        o[1] = fmaf(x[r].y, f, o[1]);
+        o[2] = fmaf(y[r].x, f, o[2]);
+        o[3] = fmaf(y[r].y, f, o[3]);
+      }
+    if (L == 0.f) L = 1.f;
+    *reinterpret_cast<float4_t *>(out_row(a, c, hk, col, D) + 4 * d4) = o / L;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Short units: 16 columns, the four waves taking the key tiles in turn and joining
+// in LDS.
+//
+// S^T = K Q^T and O^T = V^T P^T: the codes are the left operand, as they lie in
+// memory, and the weights that the first product leaves in a lane are what the
+// second one wants there.  Lane (r = lane & 15, g = lane >> 4): the left operand of
+// score product t holds, in row r, token 16 (r >> 2) + 4 t + (r & 3), dims 16 g ..
+// 16 g + 15 of each 64 (the order of the dims is free: four lanes load 64
+// neighbouring bytes), so that lane (column, g) gets the scores of tokens 16 g +
+// 4 t + i, all of one block; the left operand of the products with v holds dim
+// 16 d + r, the 16 tokens of block g.
+// The q of a lane's column, and what its scores are multiplied by.  A column
+// without a row has q 0 and is written nowhere: it sees all, so that whole tiles
+// need no mask.
 template <int D>
 struct Query {
   half8_t hi[D / 32], lo[D / 32];
   float mul;
-  int64_t see;                   // tokens that the column's row sees; 0: no row
+  int see;                       // tokens that the column's row sees
 };
 
+// The dims of lane group g are `piece` of each `step`, from piece g on (constants).
 template <int D>
-__device__ inline Query<D> load_query(const AttnArgs &a, const Columns &c, int hk, int lane) {
+__device__ inline Query<D> load_query(const AttnArgs &a, const Columns &c, int hk, int ucol,
+                                      int step, int piece) {
   Query<D> r;
-  const int col = c.base + (lane & 15), g = lane >> 4;
+  const int col = c.base + ucol, g = (threadIdx.x & 63) >> 4;
   const bool live = col < c.n * a.G;
   const int row = live ? col / a.G : 0, h = hk * a.G + (live ? col % a.G : 0);
-  const float *src = a.q + ((int64_t)(c.first + row) * a.H + h) * D + g * (D == 32 ? 8 : 16);
+  const float *src = a.q + ((int64_t)(c.first + row) * a.H + h) * D + g * piece;
   float x[D / 4];
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    const float4 v = *reinterpret_cast<const float4 *>(src + 64 * (i / 4) + 4 * (i % 4));
+    const int at = 4 * i / piece * step + 4 * i % piece;
+    const float4 v = *reinterpret_cast<const float4 *>(src + at);
     x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
   }
 #pragma unroll
@@ -142,9 +549,7 @@ __device__ inline Query<D> load_query(const AttnArgs &a, const Columns &c, int h
     if (!live) x[i] = 0.f;
     top = fmaxf(top, fabsf(x[i]));
   }
-  top = max_groups(top);
-  const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;   // 2^e <= top < 2^(e + 1)
-  const int up = min(13 - e, 120);
+  const int up = query_shift(max_groups(top));
 #pragma unroll
   for (int k = 0; k < D / 32; ++k)
 #pragma unroll
@@ -154,7 +559,7 @@ __device__ inline Query<D> load_query(const AttnArgs &a, const Columns &c, int h
       r.lo[k][j] = (_Float16)(y - (float)r.hi[k][j]);
     }
   r.mul = ldexpf(1.4426950408889634f / sqrtf((float)D), -up);
-  r.see = live ? max((int64_t)0, c.len - c.n + row + 1) : 0;
+  r.see = live ? max(0, c.len - c.n + row + 1) : INT_MAX;
   return r;
 }
 
@@ -171,7 +576,7 @@ struct State {
 // weights' halves, as the right operand of the products with v.
 template <int D, bool MASK>
 __device__ inline void softmax_tile(State<D> &s, const float4_t (&acc)[4], float ks, float vs,
-                                    float mul, int visible, half8_t (&hi)[2], half8_t (&lo)[2]) {
+                                    float lvs, float mul, int visible, half8_t (&hi)[2], half8_t (&lo)[2]) {
   const float mult = ks * mul;
   float top = -FLT_MAX;
 #pragma unroll
@@ -181,7 +586,7 @@ __device__ inline void softmax_tile(State<D> &s, const float4_t (&acc)[4], float
       top = fmaxf(top, !MASK || 4 * t + i < visible ? acc[t][i] : -FLT_MAX);
   const bool none = MASK && visible <= 0;
   const float x = none ? -INFINITY : top * mult;
-  const float xm = max_groups(x), am = max_groups(x + __builtin_amdgcn_logf(vs));
+  const float xm = max_groups(x), am = max_groups(x + lvs);
   const float m = fmaxf(s.m, ceilf(xm));
   if (__any(m != s.m)) {
     s.l *= share(s.m, m);
@@ -210,80 +615,18 @@ __device__ inline void softmax_tile(State<D> &s, const float4_t (&acc)[4], float
   for (int c = 0; c < 2; ++c) {
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float a = w[8 * c + 2 * j], b = w[8 * c + 2 * j + 1];
-      const auto x2 = __builtin_amdgcn_cvt_pkrtz(a, b);
-      h[j] = __builtin_bit_cast(uint32_t, x2);
-      l[j] = __builtin_bit_cast(uint32_t,
-                                __builtin_amdgcn_cvt_pkrtz(a - (float)x2[0], b - (float)x2[1]));
-    }
+    for (int j = 0; j < 4; ++j) split2(w[8 * c + 2 * j], w[8 * c + 2 * j + 1], h[j], l[j]);
     hi[c] = as_half8(h[0], h[1], h[2], h[3]);
     lo[c] = as_half8(l[0], l[1], l[2], l[3]);
   }
 }
 
-// ---------------------------------------------------------------------------
-// Short requests: the keys split over waves and workgroups.
-//
-// A unit is 16 columns of one request and kv head over a range of key tiles; the
-// four waves of a workgroup take its tiles in turn and join in LDS.  The range is
-// chosen so that all units together fill the chip, whatever the lengths are:
-// they are on the device, so every workgroup forms the sums over the requests
-// itself.  Where a request's keys go to several units, each leaves its state in
-// the scratch, and the last to arrive (a counter per group, left zero) joins them.
-//
-// S^T = K Q^T and O^T = V^T P^T: the codes are the left operand, as they lie in
-// memory, and the weights that the first product leaves in a lane are what the
-// second one wants there.  Lane (r = lane & 15, g = lane >> 4): the left operand of
-// score product t holds, in row r, token 16 (r >> 2) + 4 t + (r & 3), dims 16 g ..
-// 16 g + 15 of each 64 (the order of the dims is free: four lanes load 64
-// neighbouring bytes), so that lane (column, g) gets the scores of tokens 16 g +
-// 4 t + i, all of one block; the left operand of the products with v holds dim
-// 16 d + r, the 16 tokens of block g.
-constexpr int kSplitWaves = 4, kSplitThreads = kWave * kSplitWaves;
-constexpr int kSplitUnits = 512;    // units that a launch is split into, if it has the tiles
-constexpr int kSplitMin = 4;        // least tiles of a split
-
-struct Part {                        // a request's share of the work
-  int first, n, len;                 // its rows, its tokens
-  int tiles, groups;                 // tiles of keys, tiles of columns
-};
-__device__ inline Part part_of(const AttnArgs &a, int b) {
-  const RowRange r = request_rows(a.row_start, b, a.T);
-  const int len = (int)request_len(a.lens[b], a.max_blocks, a.p.lbs);
-  Part p{r.first, r.last - r.first, len, 0, 0};
-  if (p.n) {
-    p.tiles = (int)(((int64_t)len + kKeys - 1) / kKeys);
-    p.groups = (int)(((int64_t)p.n * a.G + kCols - 1) / kCols);
-  }
-  return p;
-}
-// Units of one group and kv head.
-__device__ inline int splits_of(const Part &p, int64_t chunk) {
-  return max(1, (int)((p.tiles + chunk - 1) / chunk));
-}
-
-// Sums over the 256 threads before and including `tid`; the last entry is all.
-__device__ inline int block_scan(int x, int tid, int *s_sum) {
-  const int lane = tid & 63, w = tid >> 6;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int y = __shfl_up(x, o, kWave);
-    if (lane >= o) x += y;
-  }
-  if (lane == 63) s_sum[w] = x;
-  __syncthreads();
-  for (int i = 0; i < w; ++i) x += s_sum[i];
-  __syncthreads();
-  return x;
-}
-
 template <int D>
-__device__ inline void load_k(const AttnArgs &a, const Sub &s, int hk, int lane,
+__device__ inline void load_k(const AttnArgs &a, int blk, int off, int hk, int lane,
                               uint32_t (&r)[4][D / 16]) {
   const int m = lane & 15, g = lane >> 4;
-  const int8_t *src = a.codes + head_offset(a.p, s.blk, 0, hk) +
-                      (int64_t)(s.off + (m & 3)) * D + g * (D == 32 ? 8 : 16);
+  const int8_t *src = a.codes + head_offset(a.p, blk, 0, hk) +
+                      (int64_t)(off + (m & 3)) * D + g * (D == 32 ? 8 : 16);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if constexpr (D == 32) {
@@ -300,10 +643,10 @@ __device__ inline void load_k(const AttnArgs &a, const Sub &s, int hk, int lane,
 }
 
 template <int D>
-__device__ inline void load_v(const AttnArgs &a, const Sub &s, int hk, int lane,
+__device__ inline void load_v(const AttnArgs &a, int blk, int off, int hk, int lane,
                               uint32_t (&r)[D / 16][4]) {
   const int8_t *src =
-      a.codes + head_offset(a.p, s.blk, 1, hk) + s.off + ((lane & 15) << a.p.lbs);
+      a.codes + head_offset(a.p, blk, 1, hk) + off + ((lane & 15) << a.p.lbs);
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) {
     const uint4 v = *reinterpret_cast<const uint4 *>(src + (d << (4 + a.p.lbs)));
@@ -311,316 +654,441 @@ __device__ inline void load_v(const AttnArgs &a, const Sub &s, int hk, int lane,
   }
 }
 
-// Joins the shares of a group's units, `step` floats apart: a wave at a time takes
-// a column's exponents (a lane a unit), then the threads the sums, eight units'
-// loads in flight.  lds: at least 16 x 64 floats.
 template <int D>
-__device__ inline void join(const AttnArgs &a, const Columns &c, int hk, int cols, const float *src,
-                            int64_t step, int splits, float *lds, float *s_m, float *s_l) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int col = wave; col < cols; col += kSplitWaves) {
-    float M = -INFINITY, L = 0.f;
-    for (int s = lane; s < splits; s += kWave) M = fmaxf(M, src[s * step + col * (D + 2) + D]);
+struct ShortMem {
+  float o[kShortWaves][kCols][D + 4], m[kShortWaves][kCols], l[kShortWaves][kCols], e[kShortWaves][kCols];
+};
+
+template <int D>
+__device__ inline void short_scores(const uint32_t (&kr)[4][D / 16], const Query<D> &q,
+                                    float4_t (&acc)[4]) {
 #pragma unroll
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
-    for (int s = lane; s < splits; s += kWave) {
-      const float *p = src + s * step + col * (D + 2) + D;
-      L = fmaf(p[1], share(p[0], M), L);
-    }
+  for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, kWave);
-    if (lane == 0) {
-      s_m[col] = M;
-      s_l[col] = L == 0.f ? 1.f : L;
+    for (int i = 0; i < 4; ++i) {
+      const half8_t x = codes8(kr[i][2 * j], kr[i][2 * j + 1]);
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[j], acc[i], 0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[j], acc[i], 0, 0, 0);
     }
+}
+template <int D>
+__device__ inline void short_sums(const uint32_t (&vr)[D / 16][4], const half8_t (&hi)[2],
+                                  const half8_t (&lo)[2], State<D> &st) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const half8_t x = codes8(vr[i][2 * j], vr[i][2 * j + 1]);
+      st.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi[j], st.o[i], 0, 0, 0);
+      st.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo[j], st.o[i], 0, 0, 0);
+    }
+}
+
+template <int D>
+__device__ inline void short_unit(const AttnArgs &a, const Columns &c, const Pick &u, int hk,
+                                  int chunk, float *share_at, ShortMem<D> &s) {
+  const int tid = thread_here(), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, m4 = (lane & 15) >> 2;
+  // key tiles of the unit: of the last row's tokens at most
+  const int cols = min(kCols, c.n * a.G - c.base);
+  const int most = seen_by(c.len, c.n, c.base + cols - 1, a.G);
+  const int least =                  // seen by every column
+      __builtin_amdgcn_readfirstlane(seen_by(c.len, c.n, c.base, a.G));
+  const int start = u.range * chunk;
+  // (through a division, which leaves it in a vector register)
+  const int end = __builtin_amdgcn_readfirstlane(
+      min(start + chunk, (most + kKeys - 1) / kKeys));
+  State<D> st;
+  int t = start + wave;
+  if (t < end) {
+    uint32_t kr[4][D / 16], vr[D / 16][4];
+    // places of the tile's tokens 16 m4 (k) and 16 g (v, scales) in their blocks
+    auto place = [&](int tile, int sub) { return (tile * kKeys + 16 * sub) & (a.p.bs - 1); };
+    Held held = held_tiles(a, c.table, t, kShortWaves, c.len, hk);
+    int at = 0, vblk = __shfl(held.blk, g, kWave);
+    load_k<D>(a, __shfl(held.blk, m4, kWave), place(t, m4), hk, lane, kr);
+    load_v<D>(a, vblk, place(t, g), hk, lane, vr);
+    const Query<D> q = load_query<D>(a, c, hk, lane & 15, D == 32 ? 32 : 64, D == 32 ? 8 : 16);
+    for (; t + kShortWaves < end; t += kShortWaves) {
+      const float ks = __shfl(held.ks, 4 * at + g, kWave), vs = __shfl(held.vs, 4 * at + g, kWave);
+      const float lvs = __shfl(held.lvs, 4 * at + g, kWave);
+      if (++at == kHeld) {
+        held = held_tiles(a, c.table, t + kShortWaves, kShortWaves, c.len, hk);
+        at = 0;
+      }
+      const int kblk = __shfl(held.blk, 4 * at + m4, kWave);
+      vblk = __shfl(held.blk, 4 * at + g, kWave);
+      float4_t acc[4] = {};
+      short_scores<D>(kr, q, acc);
+      load_k<D>(a, kblk, place(t + kShortWaves, m4), hk, lane, kr);
+      half8_t hi[2], lo[2];
+      if ((t + 1) * kKeys <= least)
+        softmax_tile<D, false>(st, acc, ks, vs, lvs, q.mul, 16, hi, lo);
+      else
+        softmax_tile<D, true>(st, acc, ks, vs, lvs, q.mul, min(q.see - t * kKeys, kKeys) - 16 * g,
+                              hi, lo);
+      short_sums<D>(vr, hi, lo, st);
+      load_v<D>(a, vblk, place(t + kShortWaves, g), hk, lane, vr);
+    }
+    // the last tile on its own: a condition on the loads within the loop would
+    // have them all waited for
+    float4_t acc[4] = {};
+    half8_t hi[2], lo[2];
+    short_scores<D>(kr, q, acc);
+    softmax_tile<D, true>(st, acc, __shfl(held.ks, 4 * at + g, kWave),
+                          __shfl(held.vs, 4 * at + g, kWave), __shfl(held.lvs, 4 * at + g, kWave),
+                          q.mul, min(q.see - t * kKeys, kKeys) - 16 * g, hi, lo);
+    short_sums<D>(vr, hi, lo, st);
+  }
+  // the four waves' states, then the columns' results or the unit's share of them
+  const int col = lane & 15;
+  st.l = sum_groups(st.l);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+    *reinterpret_cast<float4_t *>(&s.o[wave][col][16 * i + 4 * g]) = st.o[i];
+  if (g == 0) {
+    s.m[wave][col] = st.m;
+    s.l[wave][col] = st.l;
+    s.e[wave][col] = st.E;
   }
   __syncthreads();
-  constexpr int kTasks = kCols * D / 4, kPer = (kTasks + kSplitThreads - 1) / kSplitThreads;
-  const int tasks = cols * (D / 4);
-  float4_t o[kPer] = {};
-  for (int s0 = 0; s0 < splits; s0 += kWave) {
-    const int n = min(kWave, splits - s0);
-    for (int i = tid; i < cols * kWave; i += kSplitThreads) {
-      const int col = i / kWave, s = i % kWave;
-      lds[i] = s < n ? share(src[(s0 + s) * step + col * (D + 2) + D], s_m[col]) : 0.f;
+  for (int i = tid; i < cols * (D / 4); i += (kShortWaves * kWave)) {
+    const int cc = i / (D / 4), d4 = i % (D / 4);
+    float M = s.m[0][cc];
+#pragma unroll
+    for (int w = 1; w < kShortWaves; ++w) M = fmaxf(M, s.m[w][cc]);
+    float L = 0.f;
+    float4_t o = {};
+#pragma unroll
+    for (int w = 0; w < kShortWaves; ++w) {
+      L += s.l[w][cc] * share(s.m[w][cc], M);
+      const float4_t x = *reinterpret_cast<const float4_t *>(&s.o[w][cc][4 * d4]);
+      const int e = (int)(s.e[w][cc] - M) - 15;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += ldexpf(x[k], e);
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int i = tid + k * kSplitThreads, col = i / (D / 4);
-      if (i >= tasks) continue;
-      const float *at = src + s0 * step + col * (D + 2) + 4 * (i % (D / 4));
-      for (int s = 0; s < n; s += 8) {
-        float2 x[8], y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float *q = at + min(s + e, n - 1) * step;
-          x[e] = *reinterpret_cast<const float2 *>(q);
-          y[e] = *reinterpret_cast<const float2 *>(q + 2);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (s + e < n) {
-            const float f = lds[col * kWave + s + e];
-            o[k][0] = fmaf(x[e].x, f, o[k][0]);
-            o[k][1] = fmaf(x[e].y, f, o[k][1]);
-            o[k][2] = fmaf(y[e].x, f, o[k][2]);
-            o[k][3] = fmaf(y[e].y, f, o[k][3]);
-          }
-      }
+    if (u.ranges > 1) {
+      float *dst = share_at + cc * (D + 2);
+      put2(dst + 4 * d4, o[0], o[1]);
+      put2(dst + 4 * d4 + 2, o[2], o[3]);
+      if (d4 == 0) put2(dst + D, M, L);
+    } else {
+      if (L == 0.f) L = 1.f;           // no token is seen: the sums are 0
+      *reinterpret_cast<float4_t *>(out_row(a, c, hk, cc, D) + 4 * d4) = o / L;
     }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int i = tid + k * kSplitThreads, col = i / (D / 4), x = c.base + col;
-    if (i < tasks)
-      *reinterpret_cast<float4_t *>(
-          a.out + ((int64_t)(c.first + x / a.G) * a.H + hk * a.G + x % a.G) * D +
-          4 * (i % (D / 4))) = o[k] / s_l[col];
   }
 }
 
-__device__ inline void put2(float *p, float x, float y) {
-  const uint64_t bits = ((uint64_t)__float_as_uint(y) << 32) | __float_as_uint(x);
-  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), bits, __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
+// ---------------------------------------------------------------------------
+// Tall units: 128 columns, 16 a wave, over key tiles in LDS.
+//
+// The workgroup turns a tile's codes into halves once (two buffers: the next tile's
+// codes are loaded while a tile is worked on) and its waves read them as left
+// operands.  Row r of score product t is token 16 t + r, so lane (column, g) gets
+// the scores of tokens 16 t + 4 g + i, and the products with v take 32 tokens a step
+// in the order 4 g + i, 16 + 4 g + i, in which v is laid out.  A row has 16 bytes
+// more than its halves: 16 rows' pieces lie in different banks, at offsets that are
+// constants.  All columns see the same blocks: a scale is the same for the wave.
+template <int D>
+struct TallMem {
+  uint4 k[2][kKeys][D / 8 + 1];        // [token][8 dims]
+  uint4 v[2][D][8 + 1];                // [dim][32 tokens: g]
+};
+
+__device__ inline uint4 as_u4(half8_t x) { return __builtin_bit_cast(uint4, x); }
+__device__ inline half8_t as_half8(uint4 x) { return __builtin_bit_cast(half8_t, x); }
+__device__ inline float lane_of(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+// The codes of a tile that a thread brings: an eighth of a token's dims of k, and,
+// of v, 16 tokens of a dim (the first 4 D threads).
+template <int D>
+struct TallLoad { uint32_t k[D / 32], v[4]; };
+template <int D>
+__device__ inline void tall_load(const AttnArgs &a, int hk, int kblk, int koff, int vblk, int voff,
+                                 TallLoad<D> &r) {
+  const int tid = thread_here();
+  const int8_t *kp = a.codes + head_offset(a.p, kblk, 0, hk) +
+                     (int64_t)(koff + ((tid >> 3) & 15)) * D + (tid & 7) * (D / 8);
+  if constexpr (D == 32) {
+    r.k[0] = *reinterpret_cast<const uint32_t *>(kp);
+  } else if constexpr (D == 64) {
+    const uint2 x = *reinterpret_cast<const uint2 *>(kp);
+    r.k[0] = x.x; r.k[1] = x.y;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4 *>(kp);
+    r.k[0] = x.x; r.k[1] = x.y; r.k[2] = x.z; r.k[3] = x.w;
+  }
+  if (tid < 4 * D) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(
+        a.codes + head_offset(a.p, vblk, 1, hk) + voff + ((tid >> 2) << a.p.lbs));
+    r.v[0] = x.x; r.v[1] = x.y; r.v[2] = x.z; r.v[3] = x.w;
+  }
 }
 template <int D>
-__global__ __launch_bounds__(kSplitThreads, 2) void attn_paged_split_kernel(
-    AttnArgs a, float *__restrict__ part, unsigned *__restrict__ tickets) {
-  constexpr int kOut = D + 4;        // a column's sums in LDS
-  __shared__ float s_o[kSplitWaves][kCols][kOut];
-  __shared__ float s_m[kSplitWaves][kCols], s_l[kSplitWaves][kCols], s_e[kSplitWaves][kCols];
-  __shared__ int s_pick[12], s_sum[kSplitWaves];
-  __shared__ int64_t s_tiles[2][kSplitWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int Hkv = a.p.Hkv, per = (a.B + kSplitThreads - 1) / kSplitThreads;
-  const int b0 = tid * per, b1 = min(a.B, b0 + per);
-  // up to 256 requests: one a thread, read once
-  const Part only = b0 < b1 ? part_of(a, b0) : Part{0, 0, 0, 0, 0};
-  auto part_at = [&](int b) { return b == b0 ? only : part_of(a, b); };
-  int64_t work = 0, groups = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Part p = part_at(b);
-    work += (int64_t)p.tiles * p.groups;
-    groups += p.groups;
-  }
+__device__ inline void tall_store(TallMem<D> &s, int buf, const TallLoad<D> &r) {
+  const int tid = thread_here(), token = tid >> 3, c8 = tid & 7;
+  if constexpr (D == 32) {
+    const half8_t x = codes8(r.k[0], 0);
+    reinterpret_cast<uint2 *>(s.k[buf][token])[c8] = make_uint2(as_u4(x).x, as_u4(x).y);
+  } else {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    work += __shfl_xor(work, o, kWave);
-    groups += __shfl_xor(groups, o, kWave);
+    for (int i = 0; i < D / 64; ++i)
+      s.k[buf][token][D / 64 * c8 + i] = as_u4(codes8(r.k[2 * i], r.k[2 * i + 1]));
   }
-  if (lane == 0) {
-    s_tiles[0][wave] = work;
-    s_tiles[1][wave] = groups;
-  }
-  __syncthreads();
-  work = groups = 0;
-  for (int w = 0; w < kSplitWaves; ++w) {
-    work += s_tiles[0][w];
-    groups += s_tiles[1][w];
-  }
-  // a group of tiles / chunk + 1 units at most: all units run at once
-  const int64_t room = max((int64_t)kSplitUnits / 4, kSplitUnits - groups * Hkv);
-  const int64_t chunk = max((int64_t)kSplitMin, (work * Hkv + room - 1) / room);
-  int mine = 0, shared = 0, sgroups = 0;     // units of a kv head; those and groups that are split
-  for (int b = b0; b < b1; ++b) {
-    const Part p = part_at(b);
-    const int splits = splits_of(p, chunk);
-    mine += p.groups * splits;
-    if (splits > 1) {
-      shared += p.groups * splits;
-      sgroups += p.groups;
+  if (tid < 4 * D) {
+    // block b of the tile: tokens 4 g .. of it, at half b % 2 of piece 4 (b / 2) + g
+    const int b = tid & 3;
+    uint2 *row = reinterpret_cast<uint2 *>(s.v[buf][tid >> 2]) + 8 * (b >> 1) + (b & 1);
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      const uint4 x = as_u4(codes8(r.v[g], r.v[g + 1]));
+      row[2 * g] = make_uint2(x.x, x.y);
+      row[2 * g + 2] = make_uint2(x.z, x.w);
     }
   }
-  const int upto = block_scan(mine, tid, s_sum);
-  const int sat = block_scan(shared, tid, s_sum) - shared;
-  const int gat = block_scan(sgroups, tid, s_sum) - sgroups;
-  if (tid == kSplitThreads - 1) s_pick[11] = upto;
-  __syncthreads();
-  const int units = s_pick[11] * Hkv;
+}
 
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int item = u / Hkv, hk = u % Hkv;
-    // the thread whose requests hold the item looks it up
-    if (item < upto && item >= upto - mine) {
-      int at = upto - mine, sb = sat, gb = gat;
-      for (int b = b0; b < b1; ++b) {
-        const Part p = part_at(b);
-        const int splits = splits_of(p, chunk), k = p.groups * splits;
-        if (item < at + k) {
-          const int x = item - at, grp = x / splits;
-          s_pick[0] = b;
-          s_pick[1] = grp;
-          s_pick[2] = x % splits;
-          s_pick[3] = splits;
-          s_pick[4] = p.tiles;
-          s_pick[5] = sb + x;
-          s_pick[6] = gb + grp;
-          s_pick[8] = p.first;
-          s_pick[9] = p.n;
-          s_pick[10] = p.len;
-          break;
-        }
-        at += k;
-        if (splits > 1) {
-          sb += k;
-          gb += p.groups;
-        }
-      }
+// A tile's scales, in scalar registers.
+struct Scales { float ks[4], vs[4], lvs[4]; };
+__device__ inline Scales scales_of(const Held &h, int at) {
+  Scales s;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    s.ks[b] = lane_of(h.ks, 4 * at + b);
+    s.vs[b] = lane_of(h.vs, 4 * at + b);
+    s.lvs[b] = lane_of(h.lvs, 4 * at + b);
+  }
+  return s;
+}
+
+// Scores, softmax and products with v of a tile.  visible: tokens of the tile that
+// the lane's column sees, counted from the lane's first one.
+template <int D, bool MASK>
+__device__ inline void tall_tile(const TallMem<D> &s, int buf, const Scales &sc, const Query<D> &q,
+                                 State<D> &st, int visible) {
+  const int lane = thread_here() & 63, r = lane & 15, g = lane >> 4;
+  float4_t acc[4] = {};
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const half8_t x = as_half8(s.k[buf][16 * t + r][4 * k + g]);
+      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[k], acc[t], 0, 0, 0);
+      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[k], acc[t], 0, 0, 0);
     }
+  float ks[4], xm = -INFINITY, am = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    ks[t] = sc.ks[t] * q.mul;
+    float top = -FLT_MAX;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      top = fmaxf(top, !MASK || 16 * t + i < visible ? acc[t][i] : -FLT_MAX);
+    const float x = MASK && 16 * t >= visible ? -INFINITY : top * ks[t];
+    xm = fmaxf(xm, x);
+    am = fmaxf(am, x + sc.lvs[t]);
+  }
+  // unconditional: a branch around the sums would have them copied
+  const float m = fmaxf(st.m, ceilf(max_groups(xm)));
+  st.l *= share(st.m, m);
+  st.m = m;
+  const float E = fmaxf(st.E, ceilf(max_groups(am)));
+  const float f = __builtin_amdgcn_exp2f(st.E - E);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) st.o[i] *= f;
+  st.E = E;
+  const float base = m == -INFINITY ? 0.f : m;
+  const int shift = (int)(base - E) + 15;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float factor = fminf(ldexpf(sc.vs[2 * c + t], shift), FLT_MAX);
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = __builtin_amdgcn_exp2f(fmaf(acc[2 * c + t][i], ks[2 * c + t], -base));
+        if (MASK && 16 * (2 * c + t) + i >= visible) x = 0.f;
+        st.l += x;
+        w[i] = x * factor;
+      }
+      split2(w[0], w[1], h[2 * t], l[2 * t]);
+      split2(w[2], w[3], h[2 * t + 1], l[2 * t + 1]);
+    }
+    const half8_t hi = as_half8(h[0], h[1], h[2], h[3]), lo = as_half8(l[0], l[1], l[2], l[3]);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const half8_t x = as_half8(s.v[buf][16 * i + r][4 * c + g]);
+      st.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, st.o[i], 0, 0, 0);
+      st.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, st.o[i], 0, 0, 0);
+    }
+  }
+}
+
+template <int D>
+__device__ inline void tall_unit(const AttnArgs &a, const Columns &c, const Pick &u, int hk,
+                                 int chunk, float *share_at, TallMem<D> &s) {
+  const int tid = thread_here(), lane = tid & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cols = min(kTallCols, c.n * a.G - c.base);
+  const int col = kCols * wave + (lane & 15);
+  // tokens that the unit's last column, and the wave's last and first ones see
+  const bool any = kCols * wave < cols;
+  auto seen = [&](int x) { return seen_by(c.len, c.n, c.base + x, a.G); };
+  const int start = u.range * chunk;
+  const int end = __builtin_amdgcn_readfirstlane(
+      min(start + chunk, (seen(cols - 1) + kKeys - 1) / kKeys));
+  const int most = __builtin_amdgcn_readfirstlane(
+      any ? seen(min(cols, kCols * wave + kCols) - 1) : 0);
+  const int least = __builtin_amdgcn_readfirstlane(any ? seen(kCols * wave) : 0);
+  State<D> st;
+  if (start < end) {
+    TallLoad<D> r;
+    const int kt = 16 * (wave >> 1), vt = 16 * (tid & 3);   // the thread's tokens of a tile
+    auto load = [&](const Held &h, int at, int tile) {
+      const int tok = tile * kKeys, m = a.p.bs - 1;
+      tall_load<D>(a, hk, __builtin_amdgcn_readlane(h.blk, 4 * at + (wave >> 1)), (tok + kt) & m,
+                   __shfl(h.blk, 4 * at + (tid & 3), kWave), (tok + vt) & m, r);
+    };
+    Held held = held_tiles(a, c.table, start, 1, c.len, hk);
+    int at = 0;
+    load(held, 0, start);
+    const Query<D> q = load_query<D>(a, c, hk, col, 32, 8);
+    tall_store<D>(s, 0, r);
     __syncthreads();
-    const int b = s_pick[0], grp = s_pick[1], split = s_pick[2], splits = s_pick[3];
-    const int tiles = s_pick[4], slot = s_pick[5] * Hkv + hk, group = s_pick[6] * Hkv + hk;
-    const Columns c{s_pick[8], s_pick[9], grp * kCols, s_pick[10]};
-    // key tiles of the unit: of the last row's tokens at most
-    const int cols = min(kCols, c.n * a.G - c.base);
-    const int64_t most = max((int64_t)0, c.len - c.n + (c.base + cols - 1) / a.G + 1);
-    const int64_t least = c.len - c.n + c.base / a.G + 1;   // seen by every column
-    const int t0 = (int)min((int64_t)tiles, split * chunk);
-    const int t1 = (int)min(min((int64_t)tiles, (split + 1) * chunk), (most + kKeys - 1) / kKeys);
-    const int32_t *table = a.tables + (int64_t)b * a.max_blocks;
-    const int g = lane >> 4, m4 = (lane & 15) >> 2;
-    State<D> st;
-    int t = t0 + wave;
-    if (t < t1) {
-      uint32_t kr[4][D / 16], vr[D / 16][4];
-      Sub ks = sub_of(table, (int64_t)t * kKeys + 16 * m4, c.len, a.p);
-      Sub vs = sub_of(table, (int64_t)t * kKeys + 16 * g, c.len, a.p);
-      load_k<D>(a, ks, hk, lane, kr);
-      float ksc = a.scales[scale_offset(a.p, vs.blk, 0, hk)];
-      float vsc = a.scales[scale_offset(a.p, vs.blk, 1, hk)];
-      load_v<D>(a, vs, hk, lane, vr);
-      const Query<D> q = load_query<D>(a, c, hk, lane);
-      bool bad = vs.bad;
-      for (; t < t1; t += kSplitWaves) {
-        const int64_t next = (int64_t)(t + kSplitWaves) * kKeys;
-        const bool more = t + kSplitWaves < t1;
-        if (more) {
-          ks = sub_of(table, next + 16 * m4, c.len, a.p);
-          vs = sub_of(table, next + 16 * g, c.len, a.p);
+    for (int t = start; t < end; ++t) {
+      const int buf = (t - start) & 1;
+      const Scales sc = scales_of(held, at);
+      if (t + 1 < end) {
+        if (++at == kHeld) {
+          held = held_tiles(a, c.table, t + 1, 1, c.len, hk);
+          at = 0;
         }
-        float4_t acc[4] = {};
+        load(held, at, t + 1);
+      }
+      if ((t + 1) * kKeys <= least)
+        tall_tile<D, false>(s, buf, sc, q, st, kKeys);
+      else if (t * kKeys < most)
+        tall_tile<D, true>(s, buf, sc, q, st, min(q.see - t * kKeys, kKeys) - 4 * g);
+      if (t + 1 < end) tall_store<D>(s, buf ^ 1, r);
+      __syncthreads();
+    }
+  }
+  st.l = sum_groups(st.l);
+  const int e = (int)(st.E - st.m) - 15;
+  if (col >= cols) return;
+  float *dst = u.ranges > 1 ? share_at + col * (D + 2) : out_row(a, c, hk, col, D);
+  const float L = st.l == 0.f ? 1.f : st.l;       // no token is seen: the sums are 0
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < D / 16; ++i) {
+    float4_t x;
 #pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            const half8_t x = codes8(kr[i][2 * k], kr[i][2 * k + 1]);
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[k], acc[i], 0, 0, 0);
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[k], acc[i], 0, 0, 0);
-          }
-        const float kf = scale_ok(ksc, bad), vf = scale_ok(vsc, bad);
-        if (more) {
-          load_k<D>(a, ks, hk, lane, kr);
-          ksc = a.scales[scale_offset(a.p, vs.blk, 0, hk)];
-          vsc = a.scales[scale_offset(a.p, vs.blk, 1, hk)];
-          bad = vs.bad;
-        }
-        half8_t hi[2], lo[2];
-        // a v scale that is no number makes the scores NaN too
-        const float kn = vf == vf ? kf : vf;
-        if ((int64_t)(t + 1) * kKeys <= least && cols == kCols)
-          softmax_tile<D, false>(st, acc, kn, vf, q.mul, 16, hi, lo);
+    for (int k = 0; k < 4; ++k) x[k] = ldexpf(st.o[i][k], e);
+    if (u.ranges > 1) {
+      put2(dst + 16 * i + 4 * g, x[0], x[1]);
+      put2(dst + 16 * i + 4 * g + 2, x[2], x[3]);
+    } else {
+      *reinterpret_cast<float4_t *>(dst + 16 * i + 4 * g) = x / L;
+    }
+  }
+  if (u.ranges > 1 && g == 0) put2(dst + D, st.m, st.l);
+}
+
+// The units of a workgroup, one after the other.
+template <int D, bool TALL, int WAVES, typename Mem, typename Run>
+__device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *tickets, PlanMem &plan,
+                                 Mem &mem, JoinMem &jm, Run run) {
+  constexpr int kWide = TALL ? kTallCols : kCols;
+  constexpr int64_t kShare = (int64_t)kWide * (D + 2);
+  const int Hkv = a.p.Hkv;
+  for (int64_t k0 = 0;; k0 += kAhead) {
+    const int units = __builtin_amdgcn_readfirstlane(plan_units<TALL, WAVES>(a, k0, plan));
+    const int chunk = __builtin_amdgcn_readfirstlane(plan.chunk);
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t at = place_of(k0 + k);
+      if (at >= units) continue;
+      const int hk = (int)((uint32_t)at % Hkv);
+      // the same for every lane: in scalar registers
+      auto word = [&](int i) { return __builtin_amdgcn_readfirstlane(plan.pick[k][i]); };
+      const Pick u{word(0), word(1), word(2), word(3), word(4),
+                   word(5), word(6), word(7), word(8), word(9)};
+      const Columns c{u.first, u.n, kWide * u.group, u.len, a.tables + (int64_t)u.b * a.max_blocks};
+      const Ranges<TALL> r(Part{u.first, u.n, u.len, u.groups}, chunk, a.G);
+      auto share_of = [&](int range) {
+        return scratch + ((int64_t)(u.slot + r.place(u.group, range)) * Hkv + hk) * kShare;
+      };
+      run(c, u, hk, chunk, u.ranges > 1 ? share_of(u.range) : nullptr);
+      if (u.ranges > 1 && last_of(tickets + (int64_t)u.ticket * Hkv + hk, u.ranges, &plan.last)) {
+        const int cols = min(kWide, c.n * a.G - c.base);
+        if (u.ranges <= kFew)
+          join_few<D, WAVES>(a, c, hk, cols, u.ranges, share_of);
         else
-          softmax_tile<D, true>(st, acc, kn, vf, q.mul,
-                                (int)min(q.see - (int64_t)t * kKeys, (int64_t)kKeys) - 16 * g, hi,
-                                lo);
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const half8_t x = codes8(vr[d][2 * k], vr[d][2 * k + 1]);
-            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi[k], st.o[d], 0, 0, 0);
-            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo[k], st.o[d], 0, 0, 0);
-          }
-        if (more) load_v<D>(a, vs, hk, lane, vr);
+          join<D, WAVES>(a, c, hk, cols, u.ranges, jm, share_of);
       }
+      __syncthreads();                 // the LDS is free
     }
-    // the four waves' states, then the column's result or the unit's share of it
-    const int col = lane & 15;
-    st.l = sum_groups(st.l);
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d)
-      *reinterpret_cast<float4_t *>(&s_o[wave][col][16 * d + 4 * g]) = st.o[d];
-    if (g == 0) {
-      s_m[wave][col] = st.m;
-      s_l[wave][col] = st.l;
-      s_e[wave][col] = st.E;
-    }
-    __syncthreads();
-    float *mine_part = part + (int64_t)slot * kCols * (D + 2);
-    for (int i = tid; i < cols * (D / 4); i += kSplitThreads) {
-      const int cc = i / (D / 4), d4 = i % (D / 4);
-      float M = s_m[0][cc];
-#pragma unroll
-      for (int w = 1; w < kSplitWaves; ++w) M = fmaxf(M, s_m[w][cc]);
-      float L = 0.f;
-      float4_t o = {};
-#pragma unroll
-      for (int w = 0; w < kSplitWaves; ++w) {
-        L += s_l[w][cc] * share(s_m[w][cc], M);
-        const float4_t x = *reinterpret_cast<const float4_t *>(&s_o[w][cc][4 * d4]);
-        const int e = (int)(s_e[w][cc] - M) - 15;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] += ldexpf(x[k], e);
-      }
-      if (splits > 1) {
-        float *dst = mine_part + cc * (D + 2);
-        put2(dst + 4 * d4, o[0], o[1]);
-        put2(dst + 4 * d4 + 2, o[2], o[3]);
-        if (d4 == 0) put2(dst + D, M, L);
-      } else {
-        const int x = c.base + cc;
-        if (L == 0.f) L = 1.f;       // no token is seen: the sums are 0
-        *reinterpret_cast<float4_t *>(
-            a.out + ((int64_t)(c.first + x / a.G) * a.H + hk * a.G + x % a.G) * D + 4 * d4) = o / L;
-      }
-    }
-    if (splits > 1) {
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-      if (tid == 0) s_pick[7] = atomicAdd(tickets + group, 1u) == (unsigned)splits - 1;
-      __syncthreads();
-      if (s_pick[7]) {
-        // what the others stored is read past this die's caches
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        join<D>(a, c, hk, cols, mine_part - (int64_t)split * Hkv * kCols * (D + 2),
-                (int64_t)Hkv * kCols * (D + 2), splits, &s_o[0][0][0], s_m[0], s_l[0]);
-        if (tid == 0) atomicExch(tickets + group, 0u);
-      }
-    }
-    __syncthreads();                 // s_pick and the states are free
+    if ((k0 + kAhead) * gridDim.x >= units) return;
   }
 }
 
 template <int D>
-void launch_split(hipStream_t st, const AttnArgs &a, float *part, unsigned *tickets) {
-  // as many workgroups as there can be units, up to two a CU; the rest in turn
-  const int64_t bound = (int64_t)kSplitUnits +
+__global__ __launch_bounds__(kShortWaves *kWave, 2) void attn_paged_short_kernel(
+    AttnArgs a, float *__restrict__ scratch, unsigned *__restrict__ tickets) {
+  __shared__ PlanMem s_plan;
+  __shared__ __align__(16) union { ShortMem<D> unit; JoinMem join; } s;
+  run_units<D, false, kShortWaves>(a, scratch, tickets, s_plan, s.unit, s.join,
+                                   [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
+                                     short_unit<D>(a, c, u, hk, chunk, to, s.unit);
+                                   });
+}
+
+template <int D>
+__global__ __launch_bounds__(kTallWaves *kWave, D == 128 ? 2 : 4) void attn_paged_tall_kernel(
+    AttnArgs a, float *__restrict__ scratch, unsigned *__restrict__ tickets) {
+  __shared__ PlanMem s_plan;
+  __shared__ __align__(16) union { TallMem<D> unit; JoinMem join; } s;
+  run_units<D, true, kTallWaves>(a, scratch, tickets, s_plan, s.unit, s.join,
+                                 [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
+                                   tall_unit<D>(a, c, u, hk, chunk, to, s.unit);
+                                 });
+}
+
+template <int D>
+void launch(hipStream_t st, const AttnArgs &a, float *scratch, unsigned *tickets) {
+  if (a.tall)
+    hipLaunchKernelGGL(attn_paged_tall_kernel<D>, dim3(kSlots), dim3(kTallWaves * kWave), 0, st, a,
+                       scratch, tickets);
+  // as many workgroups as there can be units, up to two a CU
+  const int64_t bound = (int64_t)kSlots +
       (((int64_t)a.T * a.G + kCols - 1) / kCols + std::min(a.B, a.T)) * a.p.Hkv;
-  const int grid = (int)std::min<int64_t>(bound, kSplitUnits);
-  hipLaunchKernelGGL(attn_paged_split_kernel<D>, dim3(grid), dim3(kSplitThreads), 0, st, a, part,
-                     tickets);
+  hipLaunchKernelGGL(attn_paged_short_kernel<D>, dim3((unsigned)std::min<int64_t>(bound, kSlots)),
+                     dim3(kShortWaves * kWave), 0, st, a, scratch, tickets);
 }
 
 }  // namespace
 
-// A launch's units that share their columns with another: fewer than 2 units for
-// kSplitUnits (a split of `tiles` over chunk has tiles / chunk + 1 < 2 tiles /
-// chunk of them), in half as many groups at most.
-int64_t attention_paged_part_elems(int D) { return (int64_t)2 * kSplitUnits * kCols * (D + 2); }
-int attention_paged_tickets() { return kSplitUnits; }
+// Units that share their group.  Short: with room = kSlots - groups, work / chunk +
+// groups of them, kSlots; with room = kShortRoom, tiles / chunk + 1 < 2 tiles / chunk
+// for each group that has several, 2 kShortRoom.  Tall: likewise 2 kSlots.
+int64_t attention_paged_part_elems(int D) {
+  return std::max((int64_t)kSlots * kCols, (int64_t)2 * kSlots * kTallCols) * (D + 2);
+}
+int attention_paged_tickets() { return kSlots; }
 
 void launch_attention_paged(hipStream_t st, const float *q, int T, const int8_t *codes,
                             const float *scales, const PagedPool &p, const int32_t *tables,
                             int max_blocks, const int32_t *row_start, const int32_t *lens, int B,
                             int H, float *out, float *part, unsigned *tickets) {
-  const AttnArgs a{q, T, codes, scales, p, tables, max_blocks, row_start, lens, B, H, H / p.Hkv,
-                   out};
-  if (p.D == 32) launch_split<32>(st, a, part, tickets);
-  else if (p.D == 64) launch_split<64>(st, a, part, tickets);
-  else launch_split<128>(st, a, part, tickets);
+  const int G = H / p.Hkv;
+  const AttnArgs a{q, T, codes, scales, p, tables, max_blocks, row_start, lens, B, H, G, out,
+                   attention_paged_tall(T, B, G)};
+  if (p.D == 32) launch<32>(st, a, part, tickets);
+  else if (p.D == 64) launch<64>(st, a, part, tickets);
+  else launch<128>(st, a, part, tickets);
   NNHIP_CHECK(hipGetLastError());
 }
 
