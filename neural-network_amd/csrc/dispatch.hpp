@@ -68,13 +68,10 @@ inline bool attention_prompt_shape(int B, int S, int H, int D, bool q8, int max_
   return waste * share <= 1.05;
 }
 
-// Paged attention: requests of at least kPagedTallFrom columns (rows times heads of
-// q a kv head) run on units of 128 columns, in a kernel that has both these and
-// the units of 16 that serve the others; a launch whose requests have few columns
-// on average runs on the kernel of the latter alone, whatever their lengths.
-constexpr int kPagedTallFrom = 64;
+// Paged attention: units of 128 columns (rows times heads of q a kv head) of a
+// request, or of 16.
 inline bool attention_paged_tall(int T, int B, int G) {
-  return (int64_t)T * G >= kPagedTallFrom && (int64_t)T * G >= (int64_t)16 * B;
+  return (int64_t)T * G >= 64 && (int64_t)T * G >= (int64_t)32 * B;
 }
 
 // fp32 products (and int8 ones of shapes the digit GEMMs do not take).  The

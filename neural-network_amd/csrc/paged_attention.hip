@@ -102,7 +102,6 @@ struct AttnArgs {
   const int32_t *row_start, *lens;
   int B, H, G;                   // G: heads of q for one of k and v
   float *out;
-  bool tall;                     // requests of many columns run in the tall kernel
 };
 
 // Blocks and scales of 16 key tiles, `step` tiles apart, a lane for each of a tile's
@@ -138,6 +137,15 @@ __device__ inline float *out_row(const AttnArgs &a, const Columns &c, int hk, in
   return a.out + ((int64_t)(c.first + x / a.G) * a.H + hk * a.G + x % a.G) * D;
 }
 
+// Two floats that a workgroup of another die reads: written through and read past
+// the die's cache.  (A fence in their place would empty the cache for the other
+// workgroups, whose keys and values lie in it: 4 x 1000 rows, 63 us with a fence
+// after the counter, @@ without.)
+__device__ inline float2 get2(const float *p) {
+  const uint64_t bits = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)bits), __uint_as_float((uint32_t)(bits >> 32)));
+}
 __device__ inline void put2(float *p, float x, float y) {
   const uint64_t bits = ((uint64_t)__float_as_uint(y) << 32) | __float_as_uint(x);
   __hip_atomic_store(reinterpret_cast<uint64_t *>(p), bits, __ATOMIC_RELAXED,
@@ -160,33 +168,34 @@ __device__ inline void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
 // Units.
 //
 // A unit is a tile of columns of one request and kv head over a range of `chunk`
-// key tiles: 128 columns where a request has at least kTallFrom of them
+// key tiles: 128 columns where the requests have many on average
 // (attn_paged_tall_kernel), else 16 (attn_paged_short_kernel).  The lengths are on
 // the device, so every workgroup forms the sums over the requests itself and takes
 // its units from them; the ranges are chosen so that the units of a launch fill the
 // chip, whatever the lengths are.  Where a group of columns has several ranges, each
 // unit leaves its state in the scratch, and the last to arrive (a counter a group,
 // left zero) joins them.
-constexpr int kShortWaves = 4, kTallWaves = 8, kMostWaves = 8;
-constexpr int kTallCols = kCols * kTallWaves, kTallFrom = kPagedTallFrom;
+constexpr int kShortWaves = 4, kTallWaves = 8;
+constexpr int kTallCols = kCols * kTallWaves;
 constexpr int kSlots = 512;              // workgroups that run at once: two a CU
+// Workgroups of the tall kernel that run at once: its registers allow one a CU for
+// 128 dims.
+__device__ inline int tall_slots(int D) { return D == 128 ? kSlots / 2 : kSlots; }
 constexpr int kShortRoom = kSlots / 4;   // least slots that are shared out by tiles
-constexpr int kShortMin = 8, kTallMin = 4;   // least tiles of a unit of several
+constexpr int kShortMin = 8, kTallMin = 16;   // least tiles of a unit of several
 
 struct Part {                            // a request's share of the work
   int first, n, len;                     // its rows, its tokens
   int groups;                            // tiles of columns
 };
-// TALL: requests of many columns, else the others (all, if no tall kernel runs).
 template <bool TALL>
 __device__ inline Part part_of(const AttnArgs &a, int b) {
   const RowRange r = request_rows(a.row_start, b, a.T);
   const int len = (int)request_len(a.lens[b], a.max_blocks, a.p.lbs);
   Part p{r.first, r.last - r.first, len, 0};
   const int64_t cols = (int64_t)p.n * a.G;
-  const bool tall = a.tall && cols >= kTallFrom;
   constexpr int kWide = TALL ? kTallCols : kCols;
-  if (tall == TALL) p.groups = (int)((cols + kWide - 1) / kWide);
+  p.groups = (int)((cols + kWide - 1) / kWide);
   return p;
 }
 __device__ inline int tiles_of(const Part &p) { return (p.len + kKeys - 1) / kKeys; }
@@ -252,28 +261,22 @@ struct Pick {                            // a unit
   int slot, ticket;                      // the request's first, for kv head 0
 };
 constexpr int kPickWords = 10;
-constexpr int kAhead = 8;                // units that a workgroup looks up at a time
 
+template <int WAVES>
 struct PlanMem {
-  int pick[kAhead][kPickWords];
-  float work[kMostWaves];
-  int sum[kMostWaves][3];
-  int chunk, last;
+  // of each thread's requests: units up to them, the first one's place in the
+  // scratch and among the counters
+  int upto[WAVES * kWave], slot[WAVES * kWave], ticket[WAVES * kWave];
+  int pick[kPickWords], sum[WAVES][3];
+  float work[WAVES];
+  int next, last;
 };
 
-// Place of the k-th unit of a workgroup in the order in which units are dealt out:
-// rounds of all workgroups, every other one backwards, so that who had a long unit
-// gets a short one next.
-__device__ inline int64_t place_of(int64_t k) {
-  const int64_t r = k * gridDim.x;
-  return r + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-}
-
-// The workgroup's units k0 .. k0 + kAhead - 1; returns the number of all units.
+struct Plan { int units, chunk; };         // of a kv head; tiles of a unit
 template <bool TALL, int WAVES>
-__device__ inline int plan_units(const AttnArgs &a, int64_t k0, PlanMem &s) {
+__device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
   constexpr int kThreads = WAVES * kWave;
-  const int tid = thread_here(), lane = tid & 63, wave = tid >> 6, Hkv = a.p.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, Hkv = a.p.Hkv;
   // a few consecutive requests a thread (one, up to as many as there are threads)
   const int per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(a.B, b0 + per);
   const Part only = b0 < b1 ? part_of<TALL>(a, b0) : Part{0, 0, 0, 0};
@@ -284,7 +287,7 @@ __device__ inline int plan_units(const AttnArgs &a, int64_t k0, PlanMem &s) {
   for (int b = b0; b < b1; ++b) {
     const Part p = part_at(b);
     const float g = (float)p.groups;
-    work += TALL ? g * (max(0, p.len - p.n) + 1) / kKeys + g * (g + 1.f) * kCols * kTallWaves / 2 /
+    work += TALL ? g * (max(0, p.len - p.n) + 1) / kKeys + g * (g + 1.f) * kTallCols / 2 /
                            (kKeys * (float)a.G) + g
                  : g * (float)tiles_of(p);
     groups += p.groups;
@@ -307,7 +310,7 @@ __device__ inline int plan_units(const AttnArgs &a, int64_t k0, PlanMem &s) {
   __syncthreads();
   // Short: work / chunk + groups units, all at once.  Tall: no unit longer than a
   // slot's part of the work, for the rows of a prompt see more and more tokens.
-  const int room = TALL ? kSlots
+  const int room = TALL ? tall_slots(a.p.D)
                         : groups < kSlots ? max(kShortRoom, kSlots - groups * Hkv) : kShortRoom;
   const float target = work * (1.f + 1.f / 8192) * Hkv / room;
   const int chunk = max(TALL ? kTallMin : kShortMin, (int)fminf(target, 1e6f) + 1);
@@ -336,52 +339,55 @@ __device__ inline int plan_units(const AttnArgs &a, int64_t k0, PlanMem &s) {
       gat += s.sum[w][2];
     }
   }
-  sat -= shares;
-  gat -= shared;
-  for (int k = 0; k < kAhead; ++k) {
-    const int64_t at = place_of(k0 + k);
-    if (at >= (int64_t)all * Hkv) continue;
-    // the thread whose requests hold the unit writes it down
-    int x = (int)((uint32_t)at / Hkv) - (upto - mine);
-    if (x < 0 || x >= mine) continue;
-    int slot = sat, ticket = gat;
-    for (int b = b0; b < b1; ++b) {
-      const Part p = part_at(b);
-      const Ranges<TALL> r(p, chunk, a.G);
-      const int units = r.units();
-      if (x >= units) {
-        x -= units;
-        slot += r.shares();
-        ticket += p.groups - r.shared;
-        continue;
-      }
-      // range by range, a prompt's last rows, which see the most, first; short
-      // groups one by one
-      int g, range = 0;
-      if (TALL) {
-        while (x >= p.groups - r.first_group(range)) x -= p.groups - r.first_group(range++);
-        g = p.groups - 1 - x;
-      } else {
-        g = x / r.count;
-        range = x % r.count;
-      }
-      int *out = s.pick[k];
-      out[0] = b;
-      out[1] = g;
-      out[2] = range;
-      out[3] = r.of_group(g);
-      out[4] = p.first;
-      out[5] = p.n;
-      out[6] = p.len;
-      out[7] = p.groups;
-      out[8] = slot;
-      out[9] = ticket + g - r.shared;
-      break;
-    }
-  }
-  if (tid == 0) s.chunk = chunk;
+  s.upto[tid] = upto;
+  s.slot[tid] = sat - shares;
+  s.ticket[tid] = gat - shared;
   __syncthreads();
-  return all * Hkv;
+  return Plan{all, chunk};
+}
+
+// The thread whose requests hold unit `item` (of a kv head) writes it down.
+template <bool TALL, int WAVES>
+__device__ inline void find_unit(const AttnArgs &a, PlanMem<WAVES> &s, int chunk, int item) {
+  constexpr int kThreads = WAVES * kWave;
+  const int tid = thread_here();
+  int x = item - (tid ? s.upto[tid - 1] : 0);
+  if (x < 0 || item >= s.upto[tid]) return;
+  const int per = (a.B + kThreads - 1) / kThreads, b1 = min(a.B, tid * per + per);
+  int slot = s.slot[tid], ticket = s.ticket[tid];
+  for (int b = tid * per; b < b1; ++b) {
+    const Part p = part_of<TALL>(a, b);
+    const Ranges<TALL> r(p, chunk, a.G);
+    const int units = r.units();
+    if (x >= units) {
+      x -= units;
+      slot += r.shares();
+      ticket += p.groups - r.shared;
+      continue;
+    }
+    // range by range, a prompt's last rows, which see the most, first; short groups
+    // one by one
+    int g, range = 0;
+    if (TALL) {
+      while (x >= p.groups - r.first_group(range)) x -= p.groups - r.first_group(range++);
+      g = p.groups - 1 - x;
+    } else {
+      g = x / r.count;
+      range = x % r.count;
+    }
+    int *out = s.pick;
+    out[0] = b;
+    out[1] = g;
+    out[2] = range;
+    out[3] = r.of_group(g);
+    out[4] = p.first;
+    out[5] = p.n;
+    out[6] = p.len;
+    out[7] = p.groups;
+    out[8] = slot;
+    out[9] = ticket + g - r.shared;
+    return;
+  }
 }
 
 // A group's units have left their shares and arrive here; whether this is the
@@ -393,8 +399,6 @@ __device__ inline bool last_of(unsigned *ticket, int ranges, int *s_last) {
   __syncthreads();
   if (!*s_last) return false;
   if (threadIdx.x == 0) atomicExch(ticket, 0u);
-  // what the others stored is read past this die's caches
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   return true;
 }
 
@@ -411,12 +415,12 @@ __device__ inline void join(const AttnArgs &a, const Columns &c, int hk, int col
     const int here = min(kCols, cols - col0);
     for (int col = wave; col < here; col += WAVES) {
       float M = -INFINITY, L = 0.f;
-      for (int r = lane; r < ranges; r += kWave) M = fmaxf(M, at(r)[(col0 + col) * (D + 2) + D]);
+      for (int r = lane; r < ranges; r += kWave) M = fmaxf(M, get2(at(r) + (col0 + col) * (D + 2) + D).x);
 #pragma unroll
       for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
       for (int r = lane; r < ranges; r += kWave) {
-        const float *p = at(r) + (col0 + col) * (D + 2) + D;
-        L = fmaf(p[1], share(p[0], M), L);
+        const float2 ml = get2(at(r) + (col0 + col) * (D + 2) + D);
+        L = fmaf(ml.y, share(ml.x, M), L);
       }
 #pragma unroll
       for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, kWave);
@@ -432,7 +436,7 @@ __device__ inline void join(const AttnArgs &a, const Columns &c, int hk, int col
       const int n = min(kWave, ranges - r0);
       for (int i = tid; i < here * kWave; i += kThreads) {
         const int col = i / kWave, r = i % kWave;
-        s.w[col][r] = r < n ? share(at(r0 + r)[(col0 + col) * (D + 2) + D], s.m[col]) : 0.f;
+        s.w[col][r] = r < n ? share(get2(at(r0 + r) + (col0 + col) * (D + 2) + D).x, s.m[col]) : 0.f;
       }
       __syncthreads();
 #pragma unroll
@@ -445,8 +449,8 @@ __device__ inline void join(const AttnArgs &a, const Columns &c, int hk, int col
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float *q = at(r0 + min(r + e, n - 1)) + off;
-            x[e] = *reinterpret_cast<const float2 *>(q);
-            y[e] = *reinterpret_cast<const float2 *>(q + 2);
+            x[e] = get2(q);
+            y[e] = get2(q + 2);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -482,9 +486,9 @@ __device__ inline void join_few(const AttnArgs &a, const Columns &c, int hk, int
 #pragma unroll
     for (int r = 0; r < kFew; ++r) {
       const float *q = at(min(r, ranges - 1)) + col * (D + 2);
-      ml[r] = *reinterpret_cast<const float2 *>(q + D);
-      x[r] = *reinterpret_cast<const float2 *>(q + 4 * d4);
-      y[r] = *reinterpret_cast<const float2 *>(q + 4 * d4 + 2);
+      ml[r] = get2(q + D);
+      x[r] = get2(q + 4 * d4);
+      y[r] = get2(q + 4 * d4 + 2);
     }
     float M = ml[0].x, L = 0.f;
 #pragma unroll
@@ -872,13 +876,17 @@ __device__ inline void tall_tile(const TallMem<D> &s, int buf, const Scales &sc,
   const int lane = thread_here() & 63, r = lane & 15, g = lane >> 4;
   float4_t acc[4] = {};
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k)
+  for (int k = 0; k < D / 32; ++k) {
+    half8_t x[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const half8_t x = as_half8(s.k[buf][16 * t + r][4 * k + g]);
-      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[k], acc[t], 0, 0, 0);
-      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[k], acc[t], 0, 0, 0);
-    }
+    for (int t = 0; t < 4; ++t) x[t] = as_half8(s.k[buf][16 * t + r][4 * k + g]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[t], q.hi[k], acc[t], 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[t], q.lo[k], acc[t], 0, 0, 0);
+  }
   float ks[4], xm = -INFINITY, am = -INFINITY;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
@@ -920,13 +928,29 @@ __device__ inline void tall_tile(const TallMem<D> &s, int buf, const Scales &sc,
       split2(w[2], w[3], h[2 * t + 1], l[2 * t + 1]);
     }
     const half8_t hi = as_half8(h[0], h[1], h[2], h[3]), lo = as_half8(l[0], l[1], l[2], l[3]);
+    constexpr int kRun = D == 32 ? 2 : 4;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const half8_t x = as_half8(s.v[buf][16 * i + r][4 * c + g]);
-      st.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, st.o[i], 0, 0, 0);
-      st.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, st.o[i], 0, 0, 0);
+    for (int i0 = 0; i0 < D / 16; i0 += kRun) {
+      half8_t x[kRun];
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) x[i] = as_half8(s.v[buf][16 * (i0 + i) + r][4 * c + g]);
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        st.o[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i], hi, st.o[i0 + i], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        st.o[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i], lo, st.o[i0 + i], 0, 0, 0);
     }
   }
+}
+
+template <int D>
+__device__ inline void tall_out(const AttnArgs &a, const Columns &c, int hk, int col, int g,
+                                const float4_t (&o)[D / 16], float l) {
+  float *dst = out_row(a, c, hk, col, D) + 4 * g;
+  const float L = l == 0.f ? 1.f : l;             // no token is seen: the sums are 0
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float4_t *>(dst + 16 * i) = o[i] / L;
 }
 
 template <int D>
@@ -980,67 +1004,116 @@ __device__ inline void tall_unit(const AttnArgs &a, const Columns &c, const Pick
   }
   st.l = sum_groups(st.l);
   const int e = (int)(st.E - st.m) - 15;
-  if (col >= cols) return;
-  float *dst = u.ranges > 1 ? share_at + col * (D + 2) : out_row(a, c, hk, col, D);
-  const float L = st.l == 0.f ? 1.f : st.l;       // no token is seen: the sums are 0
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    float4_t x;
+  for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = ldexpf(st.o[i][k], e);
-    if (u.ranges > 1) {
-      put2(dst + 16 * i + 4 * g, x[0], x[1]);
-      put2(dst + 16 * i + 4 * g + 2, x[2], x[3]);
-    } else {
-      *reinterpret_cast<float4_t *>(dst + 16 * i + 4 * g) = x / L;
+    for (int k = 0; k < 4; ++k) st.o[i][k] = ldexpf(st.o[i][k], e);
+  if (u.ranges > 1) {
+    // as the registers lie: 16 bytes a lane
+    if (!any) return;
+    float *dst = share_at + (wave * (D / 16) * kWave + lane) * 4;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      put2(dst + i * kWave * 4, st.o[i][0], st.o[i][1]);
+      put2(dst + i * kWave * 4 + 2, st.o[i][2], st.o[i][3]);
     }
+    if (g == 0) put2(share_at + kTallCols * D + 2 * col, st.m, st.l);
+  } else if (col < cols) {
+    tall_out<D>(a, c, hk, col, g, st.o, st.l);
   }
-  if (u.ranges > 1 && g == 0) put2(dst + D, st.m, st.l);
 }
 
-// The units of a workgroup, one after the other.
-template <int D, bool TALL, int WAVES, typename Mem, typename Run>
-__device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *tickets, PlanMem &plan,
-                                 Mem &mem, JoinMem &jm, Run run) {
+// A group's shares, in the order of the ranges, by the waves that have its columns.
+template <int D, typename At>
+__device__ inline void tall_join(const AttnArgs &a, const Columns &c, int hk, int cols, int ranges,
+                                 At at) {
+  const int lane = thread_here() & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(thread_here() >> 6);
+  const int col = kCols * wave + (lane & 15);
+  if (kCols * wave >= cols) return;
+  float M = -INFINITY, L = 0.f;
+  for (int r = g; r < ranges; r += 4) M = fmaxf(M, get2(at(r) + kTallCols * D + 2 * col).x);
+  M = max_groups(M);
+  float4_t o[D / 16] = {};
+  constexpr int kAhead = D == 128 ? 2 : 4;       // shares whose loads are in flight
+  for (int r0 = 0; r0 < ranges; r0 += kAhead) {
+    float2 ml[kAhead], x[kAhead][D / 8];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const float *src = at(min(r0 + e, ranges - 1));
+      ml[e] = get2(src + kTallCols * D + 2 * col);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        x[e][i] = get2(src + ((wave * (D / 16) + i / 2) * kWave + lane) * 4 + 2 * (i % 2));
+    }
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (r0 + e >= ranges) break;
+      const float f = share(ml[e].x, M);
+      L = fmaf(ml[e].y, f, L);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i / 2][2 * (i % 2)] = fmaf(x[e][i].x, f, o[i / 2][2 * (i % 2)]);
+        o[i / 2][2 * (i % 2) + 1] = fmaf(x[e][i].y, f, o[i / 2][2 * (i % 2) + 1]);
+      }
+    }
+  }
+  if (col < cols) tall_out<D>(a, c, hk, col, g, o, L);
+}
+
+// The units of a workgroup: its own one first, then from a queue, which the last
+// workgroup to end leaves empty.  queue[0]: units taken, queue[1]: workgroups that
+// have ended.
+template <int D, bool TALL, int WAVES, typename Run>
+__device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *tickets,
+                                 PlanMem<WAVES> &s, JoinMem &jm, Run run) {
   constexpr int kWide = TALL ? kTallCols : kCols;
   constexpr int64_t kShare = (int64_t)kWide * (D + 2);
+  unsigned *queue = tickets + kSlots;
   const int Hkv = a.p.Hkv;
-  for (int64_t k0 = 0;; k0 += kAhead) {
-    const int units = __builtin_amdgcn_readfirstlane(plan_units<TALL, WAVES>(a, k0, plan));
-    const int chunk = __builtin_amdgcn_readfirstlane(plan.chunk);
-    for (int k = 0; k < kAhead; ++k) {
-      const int64_t at = place_of(k0 + k);
-      if (at >= units) continue;
-      const int hk = (int)((uint32_t)at % Hkv);
-      // the same for every lane: in scalar registers
-      auto word = [&](int i) { return __builtin_amdgcn_readfirstlane(plan.pick[k][i]); };
-      const Pick u{word(0), word(1), word(2), word(3), word(4),
-                   word(5), word(6), word(7), word(8), word(9)};
-      const Columns c{u.first, u.n, kWide * u.group, u.len, a.tables + (int64_t)u.b * a.max_blocks};
-      const Ranges<TALL> r(Part{u.first, u.n, u.len, u.groups}, chunk, a.G);
-      auto share_of = [&](int range) {
-        return scratch + ((int64_t)(u.slot + r.place(u.group, range)) * Hkv + hk) * kShare;
-      };
-      run(c, u, hk, chunk, u.ranges > 1 ? share_of(u.range) : nullptr);
-      if (u.ranges > 1 && last_of(tickets + (int64_t)u.ticket * Hkv + hk, u.ranges, &plan.last)) {
-        const int cols = min(kWide, c.n * a.G - c.base);
-        if (u.ranges <= kFew)
-          join_few<D, WAVES>(a, c, hk, cols, u.ranges, share_of);
-        else
-          join<D, WAVES>(a, c, hk, cols, u.ranges, jm, share_of);
-      }
-      __syncthreads();                 // the LDS is free
+  const Plan plan = make_plan<TALL, WAVES>(a, s);
+  const int chunk = __builtin_amdgcn_readfirstlane(plan.chunk);
+  const unsigned units = __builtin_amdgcn_readfirstlane(plan.units * Hkv);
+  unsigned at = blockIdx.x;
+  while (at < units) {
+    find_unit<TALL, WAVES>(a, s, chunk, at / Hkv);
+    if (threadIdx.x == 0) s.next = gridDim.x + (units > gridDim.x ? atomicAdd(queue, 1u) : 0u);
+    __syncthreads();
+    const int hk = at % Hkv;
+    // the same for every lane: in scalar registers
+    auto word = [&](int i) { return __builtin_amdgcn_readfirstlane(s.pick[i]); };
+    const Pick u{word(0), word(1), word(2), word(3), word(4),
+                 word(5), word(6), word(7), word(8), word(9)};
+    const Columns c{u.first, u.n, kWide * u.group, u.len, a.tables + (int64_t)u.b * a.max_blocks};
+    const Ranges<TALL> r(Part{u.first, u.n, u.len, u.groups}, chunk, a.G);
+    auto share_of = [&](int range) {
+      return scratch + ((int64_t)(u.slot + r.place(u.group, range)) * Hkv + hk) * kShare;
+    };
+    run(c, u, hk, chunk, u.ranges > 1 ? share_of(u.range) : nullptr);
+    if (u.ranges > 1 && last_of(tickets + (int64_t)u.ticket * Hkv + hk, u.ranges, &s.last)) {
+      const int cols = min(kWide, c.n * a.G - c.base);
+      if (TALL)
+        tall_join<D>(a, c, hk, cols, u.ranges, share_of);
+      else if (u.ranges <= kFew)
+        join_few<D, WAVES>(a, c, hk, cols, u.ranges, share_of);
+      else
+        join<D, WAVES>(a, c, hk, cols, u.ranges, jm, share_of);
     }
-    if ((k0 + kAhead) * gridDim.x >= units) return;
+    at = __builtin_amdgcn_readfirstlane(s.next);
+    __syncthreads();                   // the LDS is free
+  }
+  if (units > gridDim.x && threadIdx.x == 0 && atomicAdd(queue + 1, 1u) == gridDim.x - 1) {
+    atomicExch(queue, 0u);
+    atomicExch(queue + 1, 0u);
   }
 }
 
 template <int D>
 __global__ __launch_bounds__(kShortWaves *kWave, 2) void attn_paged_short_kernel(
     AttnArgs a, float *__restrict__ scratch, unsigned *__restrict__ tickets) {
-  __shared__ PlanMem s_plan;
+  __shared__ PlanMem<kShortWaves> s_plan;
   __shared__ __align__(16) union { ShortMem<D> unit; JoinMem join; } s;
-  run_units<D, false, kShortWaves>(a, scratch, tickets, s_plan, s.unit, s.join,
+  run_units<D, false, kShortWaves>(a, scratch, tickets, s_plan, s.join,
                                    [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
                                      short_unit<D>(a, c, u, hk, chunk, to, s.unit);
                                    });
@@ -1049,9 +1122,9 @@ __global__ __launch_bounds__(kShortWaves *kWave, 2) void attn_paged_short_kernel
 template <int D>
 __global__ __launch_bounds__(kTallWaves *kWave, D == 128 ? 2 : 4) void attn_paged_tall_kernel(
     AttnArgs a, float *__restrict__ scratch, unsigned *__restrict__ tickets) {
-  __shared__ PlanMem s_plan;
+  __shared__ PlanMem<kTallWaves> s_plan;
   __shared__ __align__(16) union { TallMem<D> unit; JoinMem join; } s;
-  run_units<D, true, kTallWaves>(a, scratch, tickets, s_plan, s.unit, s.join,
+  run_units<D, true, kTallWaves>(a, scratch, tickets, s_plan, s.join,
                                  [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
                                    tall_unit<D>(a, c, u, hk, chunk, to, s.unit);
                                  });
@@ -1059,9 +1132,11 @@ __global__ __launch_bounds__(kTallWaves *kWave, D == 128 ? 2 : 4) void attn_page
 
 template <int D>
 void launch(hipStream_t st, const AttnArgs &a, float *scratch, unsigned *tickets) {
-  if (a.tall)
+  if (attention_paged_tall(a.T, a.B, a.G)) {
     hipLaunchKernelGGL(attn_paged_tall_kernel<D>, dim3(kSlots), dim3(kTallWaves * kWave), 0, st, a,
                        scratch, tickets);
+    return;
+  }
   // as many workgroups as there can be units, up to two a CU
   const int64_t bound = (int64_t)kSlots +
       (((int64_t)a.T * a.G + kCols - 1) / kCols + std::min(a.B, a.T)) * a.p.Hkv;
@@ -1077,15 +1152,14 @@ void launch(hipStream_t st, const AttnArgs &a, float *scratch, unsigned *tickets
 int64_t attention_paged_part_elems(int D) {
   return std::max((int64_t)kSlots * kCols, (int64_t)2 * kSlots * kTallCols) * (D + 2);
 }
-int attention_paged_tickets() { return kSlots; }
+int attention_paged_tickets() { return kSlots + 2; }
 
 void launch_attention_paged(hipStream_t st, const float *q, int T, const int8_t *codes,
                             const float *scales, const PagedPool &p, const int32_t *tables,
                             int max_blocks, const int32_t *row_start, const int32_t *lens, int B,
                             int H, float *out, float *part, unsigned *tickets) {
   const int G = H / p.Hkv;
-  const AttnArgs a{q, T, codes, scales, p, tables, max_blocks, row_start, lens, B, H, G, out,
-                   attention_paged_tall(T, B, G)};
+  const AttnArgs a{q, T, codes, scales, p, tables, max_blocks, row_start, lens, B, H, G, out};
   if (p.D == 32) launch<32>(st, a, part, tickets);
   else if (p.D == 64) launch<64>(st, a, part, tickets);
   else launch<128>(st, a, part, tickets);
