@@ -74,6 +74,13 @@ inline bool attention_paged_tall(int T, int B, int G) {
   return (int64_t)T * G >= 64 && (int64_t)T * G >= (int64_t)32 * B;
 }
 
+// Units of 16 columns, with a wave each or with four: `groups` estimates how many
+// there are.
+inline bool attention_paged_solo(int T, int B, int G, int Hkv) {
+  const int64_t groups = std::max<int64_t>(((int64_t)T * G + 15) / 16, std::min(T, B));
+  return groups * Hkv >= 1024;
+}
+
 // fp32 products (and int8 ones of shapes the digit GEMMs do not take).  The
 // fp32 MFMA GEMM takes the GEMV over from 16 rows and 90000 outputs on: the
 // GEMV runs at about 20 TFLOP/s, the GEMM costs 7 ns per entry of K and wave

@@ -182,6 +182,9 @@ constexpr int kSlots = 512;              // workgroups that run at once: two a C
 // 128 dims.
 __device__ inline int tall_slots(int D) { return D == 128 ? kSlots / 2 : kSlots; }
 constexpr int kShortRoom = kSlots / 4;   // least slots that are shared out by tiles
+constexpr int kSoloSlots = kSlots * kShortWaves;
+constexpr int kTickets = kSoloSlots;     // counters of groups, then the queue's two
+enum { kShort, kSolo, kTall };
 constexpr int kShortMin = 8, kTallMin = 16;   // least tiles of a unit of several
 
 struct Part {                            // a request's share of the work
@@ -239,6 +242,7 @@ struct Ranges {
   }
   // place of (group g, range s) among the request's shares, range by range
   __device__ int place(int g, int s) const {
+    if (!TALL) return s * groups + g;
     int at = 0;
     for (int i = 0; i < s; ++i) at += groups - max(shared, first_group(i));
     return at + g - max(shared, first_group(s));
@@ -257,25 +261,26 @@ __device__ inline int wave_scan(int x) {
 }
 
 struct Pick {                            // a unit
-  int b, group, range, ranges, first, n, len, groups;
-  int slot, ticket;                      // the request's first, for kv head 0
+  int b, group, range, ranges;
+  Part part;
+  int slot, ticket;                      // of its shares' first, its counter; for kv head 0
 };
-constexpr int kPickWords = 10;
 
 template <int WAVES>
 struct PlanMem {
   // of each thread's requests: units up to them, the first one's place in the
   // scratch and among the counters
   int upto[WAVES * kWave], slot[WAVES * kWave], ticket[WAVES * kWave];
-  int pick[kPickWords], sum[WAVES][3];
+  int sum[WAVES][3];
   float work[WAVES];
   int next, last;
 };
 
 struct Plan { int units, chunk; };         // of a kv head; tiles of a unit
-template <bool TALL, int WAVES>
+template <int KIND, int WAVES>
 __device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
   constexpr int kThreads = WAVES * kWave;
+  constexpr bool TALL = KIND == kTall;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, Hkv = a.p.Hkv;
   // a few consecutive requests a thread (one, up to as many as there are threads)
   const int per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(a.B, b0 + per);
@@ -308,12 +313,14 @@ __device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
     groups += s.sum[w][0];
   }
   __syncthreads();
-  // Short: work / chunk + groups units, all at once.  Tall: no unit longer than a
-  // slot's part of the work, for the rows of a prompt see more and more tokens.
-  const int room = TALL ? tall_slots(a.p.D)
-                        : groups < kSlots ? max(kShortRoom, kSlots - groups * Hkv) : kShortRoom;
+  // Short: work / chunk + groups units, all at once.  Tall, solo: no unit longer than
+  // a slot's part of the work (the rows of a prompt see more and more tokens).
+  const int room = KIND == kSolo ? kSoloSlots
+                   : TALL        ? tall_slots(a.p.D)
+                   : groups < kSlots ? max(kShortRoom, kSlots - groups * Hkv)
+                                     : kShortRoom;
   const float target = work * (1.f + 1.f / 8192) * Hkv / room;
-  const int chunk = max(TALL ? kTallMin : kShortMin, (int)fminf(target, 1e6f) + 1);
+  const int chunk = max(KIND == kShort ? kShortMin : kTallMin, (int)fminf(target, 1e6f) + 1);
   int mine = 0, shares = 0, shared = 0;      // units, those that share a group, such groups
   for (int b = b0; b < b1; ++b) {
     const Part p = part_at(b);
@@ -346,15 +353,18 @@ __device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
   return Plan{all, chunk};
 }
 
-// The thread whose requests hold unit `item` (of a kv head) writes it down.
+// Unit `item` (of a kv head), the same for the whole wave.
 template <bool TALL, int WAVES>
-__device__ inline void find_unit(const AttnArgs &a, PlanMem<WAVES> &s, int chunk, int item) {
+__device__ inline Pick find_unit(const AttnArgs &a, const PlanMem<WAVES> &s, int chunk, int item) {
   constexpr int kThreads = WAVES * kWave;
-  const int tid = thread_here();
-  int x = item - (tid ? s.upto[tid - 1] : 0);
-  if (x < 0 || item >= s.upto[tid]) return;
+  const int lane = thread_here() & 63;
+  // the first thread whose requests reach beyond it
+  const uint64_t beyond = __ballot(s.upto[lane * WAVES + WAVES - 1] > item);
+  int tid = beyond ? __builtin_ctzll(beyond) * WAVES : 0;
+  while (s.upto[tid] <= item && tid < kThreads - 1) ++tid;
+  tid = __builtin_amdgcn_readfirstlane(tid);
   const int per = (a.B + kThreads - 1) / kThreads, b1 = min(a.B, tid * per + per);
-  int slot = s.slot[tid], ticket = s.ticket[tid];
+  int x = item - (tid ? s.upto[tid - 1] : 0), slot = s.slot[tid], ticket = s.ticket[tid];
   for (int b = tid * per; b < b1; ++b) {
     const Part p = part_of<TALL>(a, b);
     const Ranges<TALL> r(p, chunk, a.G);
@@ -375,19 +385,12 @@ __device__ inline void find_unit(const AttnArgs &a, PlanMem<WAVES> &s, int chunk
       g = x / r.count;
       range = x % r.count;
     }
-    int *out = s.pick;
-    out[0] = b;
-    out[1] = g;
-    out[2] = range;
-    out[3] = r.of_group(g);
-    out[4] = p.first;
-    out[5] = p.n;
-    out[6] = p.len;
-    out[7] = p.groups;
-    out[8] = slot;
-    out[9] = ticket + g - r.shared;
-    return;
+    auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    return Pick{one(b), one(g), one(range), one(r.of_group(g)),
+                Part{one(p.first), one(p.n), one(p.len), one(p.groups)}, one(slot),
+                one(ticket + g - r.shared)};
   }
+  return Pick{0, 0, 0, 0, Part{0, 0, 0, 0}, 0, 0};   // not reached: item < units
 }
 
 // A group's units have left their shares and arrive here; whether this is the
@@ -625,6 +628,73 @@ __device__ inline void softmax_tile(State<D> &s, const float4_t (&acc)[4], float
   }
 }
 
+// A wave's 16 columns: their results, or the unit's share of them, as the registers
+// lie (16 bytes a lane; the wave's part of a share of `width` columns).
+template <int D>
+__device__ inline void wave_out(const AttnArgs &a, const Columns &c, int hk, int col, int g,
+                                const float4_t (&o)[D / 16], float l) {
+  float *dst = out_row(a, c, hk, col, D) + 4 * g;
+  const float L = l == 0.f ? 1.f : l;             // no token is seen: the sums are 0
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float4_t *>(dst + 16 * i) = o[i] / L;
+}
+template <int D>
+__device__ inline void wave_end(const AttnArgs &a, const Columns &c, int hk, int col, int cols,
+                                int ranges, float *share_at, int part, int width, State<D> &st) {
+  const int lane = thread_here() & 63, g = lane >> 4;
+  st.l = sum_groups(st.l);
+  const int e = (int)(st.E - st.m) - 15;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) st.o[i][k] = ldexpf(st.o[i][k], e);
+  if (ranges > 1) {
+    float *dst = share_at + (part * (D / 16) * kWave + lane) * 4;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      put2(dst + i * kWave * 4, st.o[i][0], st.o[i][1]);
+      put2(dst + i * kWave * 4 + 2, st.o[i][2], st.o[i][3]);
+    }
+    if (g == 0) put2(share_at + width * D + 2 * col, st.m, st.l);
+  } else if (col < cols) {
+    wave_out<D>(a, c, hk, col, g, st.o, st.l);
+  }
+}
+// The shares of a group, in the order of the ranges.
+template <int D, typename At>
+__device__ inline void wave_join(const AttnArgs &a, const Columns &c, int hk, int col, int cols,
+                                 int ranges, int part, int width, At at) {
+  const int lane = thread_here() & 63, g = lane >> 4;
+  float M = -INFINITY, L = 0.f;
+  for (int r = g; r < ranges; r += 4) M = fmaxf(M, get2(at(r) + width * D + 2 * col).x);
+  M = max_groups(M);
+  float4_t o[D / 16] = {};
+  constexpr int kAhead = D == 128 ? 2 : 4;       // shares whose loads are in flight
+  for (int r0 = 0; r0 < ranges; r0 += kAhead) {
+    float2 ml[kAhead], x[kAhead][D / 8];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const float *src = at(min(r0 + e, ranges - 1));
+      ml[e] = get2(src + width * D + 2 * col);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        x[e][i] = get2(src + ((part * (D / 16) + i / 2) * kWave + lane) * 4 + 2 * (i % 2));
+    }
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (r0 + e >= ranges) break;
+      const float f = share(ml[e].x, M);
+      L = fmaf(ml[e].y, f, L);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i / 2][2 * (i % 2)] = fmaf(x[e][i].x, f, o[i / 2][2 * (i % 2)]);
+        o[i / 2][2 * (i % 2) + 1] = fmaf(x[e][i].y, f, o[i / 2][2 * (i % 2) + 1]);
+      }
+    }
+  }
+  if (col < cols) wave_out<D>(a, c, hk, col, g, o, L);
+}
+
 template <int D>
 __device__ inline void load_k(const AttnArgs &a, int blk, int off, int hk, int lane,
                               uint32_t (&r)[4][D / 16]) {
@@ -688,63 +758,68 @@ __device__ inline void short_sums(const uint32_t (&vr)[D / 16][4], const half8_t
     }
 }
 
+// The state of a wave after key tiles t, t + STEP, .. below `end`, of 16 columns.
+template <int D, int STEP>
+__device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, int t, int end,
+                                   State<D> &st) {
+  const int lane = thread_here() & 63, g = lane >> 4, m4 = (lane & 15) >> 2;
+  const int least =                  // seen by every column
+      __builtin_amdgcn_readfirstlane(seen_by(c.len, c.n, c.base, a.G));
+  if (t >= end) return;
+  uint32_t kr[4][D / 16], vr[D / 16][4];
+  // places of the tile's tokens 16 m4 (k) and 16 g (v, scales) in their blocks
+  auto place = [&](int tile, int sub) { return (tile * kKeys + 16 * sub) & (a.p.bs - 1); };
+  Held held = held_tiles(a, c.table, t, STEP, c.len, hk);
+  int at = 0, vblk = __shfl(held.blk, g, kWave);
+  load_k<D>(a, __shfl(held.blk, m4, kWave), place(t, m4), hk, lane, kr);
+  load_v<D>(a, vblk, place(t, g), hk, lane, vr);
+  const Query<D> q = load_query<D>(a, c, hk, lane & 15, D == 32 ? 32 : 64, D == 32 ? 8 : 16);
+  for (; t + STEP < end; t += STEP) {
+    const float ks = __shfl(held.ks, 4 * at + g, kWave), vs = __shfl(held.vs, 4 * at + g, kWave);
+    const float lvs = __shfl(held.lvs, 4 * at + g, kWave);
+    if (++at == kHeld) {
+      held = held_tiles(a, c.table, t + STEP, STEP, c.len, hk);
+      at = 0;
+    }
+    const int kblk = __shfl(held.blk, 4 * at + m4, kWave);
+    vblk = __shfl(held.blk, 4 * at + g, kWave);
+    float4_t acc[4] = {};
+    short_scores<D>(kr, q, acc);
+    load_k<D>(a, kblk, place(t + STEP, m4), hk, lane, kr);
+    half8_t hi[2], lo[2];
+    if ((t + 1) * kKeys <= least)
+      softmax_tile<D, false>(st, acc, ks, vs, lvs, q.mul, 16, hi, lo);
+    else
+      softmax_tile<D, true>(st, acc, ks, vs, lvs, q.mul, min(q.see - t * kKeys, kKeys) - 16 * g, hi,
+                            lo);
+    short_sums<D>(vr, hi, lo, st);
+    load_v<D>(a, vblk, place(t + STEP, g), hk, lane, vr);
+  }
+  // the last tile on its own: a condition on the loads within the loop would have
+  // them all waited for
+  float4_t acc[4] = {};
+  half8_t hi[2], lo[2];
+  short_scores<D>(kr, q, acc);
+  softmax_tile<D, true>(st, acc, __shfl(held.ks, 4 * at + g, kWave),
+                        __shfl(held.vs, 4 * at + g, kWave), __shfl(held.lvs, 4 * at + g, kWave),
+                        q.mul, min(q.see - t * kKeys, kKeys) - 16 * g, hi, lo);
+  short_sums<D>(vr, hi, lo, st);
+}
+// Key tiles of a unit: up to the last row's tokens.
+__device__ inline int end_of(const AttnArgs &a, const Columns &c, int start, int chunk, int cols) {
+  // (through a division, which leaves it in a vector register)
+  return __builtin_amdgcn_readfirstlane(
+      min(start + chunk, (seen_by(c.len, c.n, c.base + cols - 1, a.G) + kKeys - 1) / kKeys));
+}
+
 template <int D>
 __device__ inline void short_unit(const AttnArgs &a, const Columns &c, const Pick &u, int hk,
                                   int chunk, float *share_at, ShortMem<D> &s) {
-  const int tid = thread_here(), lane = tid & 63;
+  const int tid = thread_here(), lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, m4 = (lane & 15) >> 2;
-  // key tiles of the unit: of the last row's tokens at most
-  const int cols = min(kCols, c.n * a.G - c.base);
-  const int most = seen_by(c.len, c.n, c.base + cols - 1, a.G);
-  const int least =                  // seen by every column
-      __builtin_amdgcn_readfirstlane(seen_by(c.len, c.n, c.base, a.G));
-  const int start = u.range * chunk;
-  // (through a division, which leaves it in a vector register)
-  const int end = __builtin_amdgcn_readfirstlane(
-      min(start + chunk, (most + kKeys - 1) / kKeys));
+  const int cols = min(kCols, c.n * a.G - c.base), start = u.range * chunk;
   State<D> st;
-  int t = start + wave;
-  if (t < end) {
-    uint32_t kr[4][D / 16], vr[D / 16][4];
-    // places of the tile's tokens 16 m4 (k) and 16 g (v, scales) in their blocks
-    auto place = [&](int tile, int sub) { return (tile * kKeys + 16 * sub) & (a.p.bs - 1); };
-    Held held = held_tiles(a, c.table, t, kShortWaves, c.len, hk);
-    int at = 0, vblk = __shfl(held.blk, g, kWave);
-    load_k<D>(a, __shfl(held.blk, m4, kWave), place(t, m4), hk, lane, kr);
-    load_v<D>(a, vblk, place(t, g), hk, lane, vr);
-    const Query<D> q = load_query<D>(a, c, hk, lane & 15, D == 32 ? 32 : 64, D == 32 ? 8 : 16);
-    for (; t + kShortWaves < end; t += kShortWaves) {
-      const float ks = __shfl(held.ks, 4 * at + g, kWave), vs = __shfl(held.vs, 4 * at + g, kWave);
-      const float lvs = __shfl(held.lvs, 4 * at + g, kWave);
-      if (++at == kHeld) {
-        held = held_tiles(a, c.table, t + kShortWaves, kShortWaves, c.len, hk);
-        at = 0;
-      }
-      const int kblk = __shfl(held.blk, 4 * at + m4, kWave);
-      vblk = __shfl(held.blk, 4 * at + g, kWave);
-      float4_t acc[4] = {};
-      short_scores<D>(kr, q, acc);
-      load_k<D>(a, kblk, place(t + kShortWaves, m4), hk, lane, kr);
-      half8_t hi[2], lo[2];
-      if ((t + 1) * kKeys <= least)
-        softmax_tile<D, false>(st, acc, ks, vs, lvs, q.mul, 16, hi, lo);
-      else
-        softmax_tile<D, true>(st, acc, ks, vs, lvs, q.mul, min(q.see - t * kKeys, kKeys) - 16 * g,
-                              hi, lo);
-      short_sums<D>(vr, hi, lo, st);
-      load_v<D>(a, vblk, place(t + kShortWaves, g), hk, lane, vr);
-    }
-    // the last tile on its own: a condition on the loads within the loop would
-    // have them all waited for
-    float4_t acc[4] = {};
-    half8_t hi[2], lo[2];
-    short_scores<D>(kr, q, acc);
-    softmax_tile<D, true>(st, acc, __shfl(held.ks, 4 * at + g, kWave),
-                          __shfl(held.vs, 4 * at + g, kWave), __shfl(held.lvs, 4 * at + g, kWave),
-                          q.mul, min(q.see - t * kKeys, kKeys) - 16 * g, hi, lo);
-    short_sums<D>(vr, hi, lo, st);
-  }
+  short_tiles<D, kShortWaves>(a, c, hk, start + wave, end_of(a, c, start, chunk, cols), st);
   // the four waves' states, then the columns' results or the unit's share of them
   const int col = lane & 15;
   st.l = sum_groups(st.l);
@@ -945,15 +1020,6 @@ __device__ inline void tall_tile(const TallMem<D> &s, int buf, const Scales &sc,
 }
 
 template <int D>
-__device__ inline void tall_out(const AttnArgs &a, const Columns &c, int hk, int col, int g,
-                                const float4_t (&o)[D / 16], float l) {
-  float *dst = out_row(a, c, hk, col, D) + 4 * g;
-  const float L = l == 0.f ? 1.f : l;             // no token is seen: the sums are 0
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float4_t *>(dst + 16 * i) = o[i] / L;
-}
-
-template <int D>
 __device__ inline void tall_unit(const AttnArgs &a, const Columns &c, const Pick &u, int hk,
                                  int chunk, float *share_at, TallMem<D> &s) {
   const int tid = thread_here(), lane = tid & 63, g = lane >> 4;
@@ -964,8 +1030,7 @@ __device__ inline void tall_unit(const AttnArgs &a, const Columns &c, const Pick
   const bool any = kCols * wave < cols;
   auto seen = [&](int x) { return seen_by(c.len, c.n, c.base + x, a.G); };
   const int start = u.range * chunk;
-  const int end = __builtin_amdgcn_readfirstlane(
-      min(start + chunk, (seen(cols - 1) + kKeys - 1) / kKeys));
+  const int end = end_of(a, c, start, chunk, cols);
   const int most = __builtin_amdgcn_readfirstlane(
       any ? seen(min(cols, kCols * wave + kCols) - 1) : 0);
   const int least = __builtin_amdgcn_readfirstlane(any ? seen(kCols * wave) : 0);
@@ -1002,109 +1067,105 @@ __device__ inline void tall_unit(const AttnArgs &a, const Columns &c, const Pick
       __syncthreads();
     }
   }
-  st.l = sum_groups(st.l);
-  const int e = (int)(st.E - st.m) - 15;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) st.o[i][k] = ldexpf(st.o[i][k], e);
-  if (u.ranges > 1) {
-    // as the registers lie: 16 bytes a lane
-    if (!any) return;
-    float *dst = share_at + (wave * (D / 16) * kWave + lane) * 4;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      put2(dst + i * kWave * 4, st.o[i][0], st.o[i][1]);
-      put2(dst + i * kWave * 4 + 2, st.o[i][2], st.o[i][3]);
-    }
-    if (g == 0) put2(share_at + kTallCols * D + 2 * col, st.m, st.l);
-  } else if (col < cols) {
-    tall_out<D>(a, c, hk, col, g, st.o, st.l);
+  if (any) wave_end<D>(a, c, hk, col, cols, u.ranges, share_at, wave, kTallCols, st);
+}
+
+// What a unit works on.
+template <int D, bool TALL>
+struct Unit {
+  static constexpr int kWide = TALL ? kTallCols : kCols;
+  Pick u;
+  int hk, cols;
+  Columns c;
+  Ranges<TALL> r;
+  float *shares;
+  int64_t step;
+  __device__ Unit(const AttnArgs &a, const Pick &u_, int hk_, int chunk, float *scratch)
+      : u(u_), hk(hk_),
+        c{u.part.first, u.part.n, kWide * u.group, u.part.len, a.tables + (int64_t)u.b * a.max_blocks},
+        r(u.part, chunk, a.G) {
+    cols = min(kWide, c.n * a.G - c.base);
+    step = (int64_t)a.p.Hkv * kWide * (D + 2);
+    shares = scratch + u.slot * step + (int64_t)hk * kWide * (D + 2);
+  }
+  __device__ float *share_of(int range) const { return shares + r.place(u.group, range) * step; }
+};
+
+// Workgroups (solo: waves) take their own unit first, the others from a queue, which
+// the last to end leaves empty.  queue[0]: units taken, queue[1]: who has ended.
+__device__ inline void leave_queue(unsigned *queue, unsigned takers) {
+  if (atomicAdd(queue + 1, 1u) == takers - 1) {
+    atomicExch(queue, 0u);
+    atomicExch(queue + 1, 0u);
   }
 }
 
-// A group's shares, in the order of the ranges, by the waves that have its columns.
-template <int D, typename At>
-__device__ inline void tall_join(const AttnArgs &a, const Columns &c, int hk, int cols, int ranges,
-                                 At at) {
-  const int lane = thread_here() & 63, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(thread_here() >> 6);
-  const int col = kCols * wave + (lane & 15);
-  if (kCols * wave >= cols) return;
-  float M = -INFINITY, L = 0.f;
-  for (int r = g; r < ranges; r += 4) M = fmaxf(M, get2(at(r) + kTallCols * D + 2 * col).x);
-  M = max_groups(M);
-  float4_t o[D / 16] = {};
-  constexpr int kAhead = D == 128 ? 2 : 4;       // shares whose loads are in flight
-  for (int r0 = 0; r0 < ranges; r0 += kAhead) {
-    float2 ml[kAhead], x[kAhead][D / 8];
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const float *src = at(min(r0 + e, ranges - 1));
-      ml[e] = get2(src + kTallCols * D + 2 * col);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        x[e][i] = get2(src + ((wave * (D / 16) + i / 2) * kWave + lane) * 4 + 2 * (i % 2));
-    }
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      if (r0 + e >= ranges) break;
-      const float f = share(ml[e].x, M);
-      L = fmaf(ml[e].y, f, L);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i / 2][2 * (i % 2)] = fmaf(x[e][i].x, f, o[i / 2][2 * (i % 2)]);
-        o[i / 2][2 * (i % 2) + 1] = fmaf(x[e][i].y, f, o[i / 2][2 * (i % 2) + 1]);
-      }
-    }
-  }
-  if (col < cols) tall_out<D>(a, c, hk, col, g, o, L);
-}
-
-// The units of a workgroup: its own one first, then from a queue, which the last
-// workgroup to end leaves empty.  queue[0]: units taken, queue[1]: workgroups that
-// have ended.
-template <int D, bool TALL, int WAVES, typename Run>
+template <int D, int KIND, int WAVES, typename Run>
 __device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *tickets,
                                  PlanMem<WAVES> &s, JoinMem &jm, Run run) {
-  constexpr int kWide = TALL ? kTallCols : kCols;
-  constexpr int64_t kShare = (int64_t)kWide * (D + 2);
-  unsigned *queue = tickets + kSlots;
+  constexpr bool TALL = KIND == kTall;
+  unsigned *queue = tickets + kTickets;
   const int Hkv = a.p.Hkv;
-  const Plan plan = make_plan<TALL, WAVES>(a, s);
+  const Plan plan = make_plan<KIND, WAVES>(a, s);
   const int chunk = __builtin_amdgcn_readfirstlane(plan.chunk);
   const unsigned units = __builtin_amdgcn_readfirstlane(plan.units * Hkv);
   unsigned at = blockIdx.x;
   while (at < units) {
-    find_unit<TALL, WAVES>(a, s, chunk, at / Hkv);
+    const Unit<D, TALL> w(a, find_unit<TALL, WAVES>(a, s, chunk, at / Hkv), at % Hkv, chunk, scratch);
     if (threadIdx.x == 0) s.next = gridDim.x + (units > gridDim.x ? atomicAdd(queue, 1u) : 0u);
-    __syncthreads();
-    const int hk = at % Hkv;
-    // the same for every lane: in scalar registers
-    auto word = [&](int i) { return __builtin_amdgcn_readfirstlane(s.pick[i]); };
-    const Pick u{word(0), word(1), word(2), word(3), word(4),
-                 word(5), word(6), word(7), word(8), word(9)};
-    const Columns c{u.first, u.n, kWide * u.group, u.len, a.tables + (int64_t)u.b * a.max_blocks};
-    const Ranges<TALL> r(Part{u.first, u.n, u.len, u.groups}, chunk, a.G);
-    auto share_of = [&](int range) {
-      return scratch + ((int64_t)(u.slot + r.place(u.group, range)) * Hkv + hk) * kShare;
-    };
-    run(c, u, hk, chunk, u.ranges > 1 ? share_of(u.range) : nullptr);
-    if (u.ranges > 1 && last_of(tickets + (int64_t)u.ticket * Hkv + hk, u.ranges, &s.last)) {
-      const int cols = min(kWide, c.n * a.G - c.base);
-      if (TALL)
-        tall_join<D>(a, c, hk, cols, u.ranges, share_of);
-      else if (u.ranges <= kFew)
-        join_few<D, WAVES>(a, c, hk, cols, u.ranges, share_of);
-      else
-        join<D, WAVES>(a, c, hk, cols, u.ranges, jm, share_of);
+    run(w.c, w.u, w.hk, chunk, w.u.ranges > 1 ? w.share_of(w.u.range) : nullptr);
+    if (w.u.ranges > 1 && last_of(tickets + (int64_t)w.u.ticket * Hkv + w.hk, w.u.ranges, &s.last)) {
+      auto share_of = [&](int range) { return w.share_of(range); };
+      if constexpr (TALL) {
+        const int wave = __builtin_amdgcn_readfirstlane(thread_here() >> 6);
+        if (kCols * wave < w.cols)
+          wave_join<D>(a, w.c, w.hk, kCols * wave + (thread_here() & 15), w.cols, w.u.ranges, wave,
+                       kTallCols, share_of);
+      } else if (w.u.ranges <= kFew) {
+        join_few<D, WAVES>(a, w.c, w.hk, w.cols, w.u.ranges, share_of);
+      } else {
+        join<D, WAVES>(a, w.c, w.hk, w.cols, w.u.ranges, jm, share_of);
+      }
     }
+    __syncthreads();                   // s.next is there
     at = __builtin_amdgcn_readfirstlane(s.next);
     __syncthreads();                   // the LDS is free
   }
-  if (units > gridDim.x && threadIdx.x == 0 && atomicAdd(queue + 1, 1u) == gridDim.x - 1) {
-    atomicExch(queue, 0u);
-    atomicExch(queue + 1, 0u);
+  if (units > gridDim.x && threadIdx.x == 0) leave_queue(queue, gridDim.x);
+}
+
+// Units of 16 columns with a wave each, where there are so many of them that four
+// waves a unit would wait more than work.
+template <int D>
+__global__ __launch_bounds__(kShortWaves *kWave, 2) void attn_paged_solo_kernel(
+    AttnArgs a, float *__restrict__ scratch, unsigned *__restrict__ tickets) {
+  __shared__ PlanMem<kShortWaves> s;
+  const int Hkv = a.p.Hkv;
+  const Plan plan = make_plan<kSolo, kShortWaves>(a, s);
+  const int chunk = __builtin_amdgcn_readfirstlane(plan.chunk);
+  const unsigned units = __builtin_amdgcn_readfirstlane(plan.units * Hkv);
+  const unsigned takers = gridDim.x * kShortWaves;
+  // neighbouring waves of different workgroups first: few units spread over the chip
+  unsigned at = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * gridDim.x + blockIdx.x;
+  for (; at < units; at += takers) {
+    const Unit<D, false> w(a, find_unit<false, kShortWaves>(a, s, chunk, at / Hkv), at % Hkv, chunk,
+                           scratch);
+    const int col = thread_here() & 15, start = w.u.range * chunk;
+    State<D> st;
+    short_tiles<D, 1>(a, w.c, w.hk, start, end_of(a, w.c, start, chunk, w.cols), st);
+    wave_end<D>(a, w.c, w.hk, col, w.cols, w.u.ranges,
+                w.u.ranges > 1 ? w.share_of(w.u.range) : nullptr, 0, kCols, st);
+    if (w.u.ranges > 1) {
+      __builtin_amdgcn_s_waitcnt(0);
+      unsigned *ticket = tickets + (int64_t)w.u.ticket * Hkv + w.hk;
+      unsigned n = 0;
+      if ((thread_here() & 63) == 0) n = atomicAdd(ticket, 1u);
+      if (__builtin_amdgcn_readfirstlane(n) == (unsigned)w.u.ranges - 1) {
+        if ((thread_here() & 63) == 0) atomicExch(ticket, 0u);
+        wave_join<D>(a, w.c, w.hk, col, w.cols, w.u.ranges, 0, kCols,
+                     [&](int range) { return w.share_of(range); });
+      }
+    }
   }
 }
 
@@ -1113,7 +1174,7 @@ __global__ __launch_bounds__(kShortWaves *kWave, 2) void attn_paged_short_kernel
     AttnArgs a, float *__restrict__ scratch, unsigned *__restrict__ tickets) {
   __shared__ PlanMem<kShortWaves> s_plan;
   __shared__ __align__(16) union { ShortMem<D> unit; JoinMem join; } s;
-  run_units<D, false, kShortWaves>(a, scratch, tickets, s_plan, s.join,
+  run_units<D, kShort, kShortWaves>(a, scratch, tickets, s_plan, s.join,
                                    [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
                                      short_unit<D>(a, c, u, hk, chunk, to, s.unit);
                                    });
@@ -1124,7 +1185,7 @@ __global__ __launch_bounds__(kTallWaves *kWave, D == 128 ? 2 : 4) void attn_page
     AttnArgs a, float *__restrict__ scratch, unsigned *__restrict__ tickets) {
   __shared__ PlanMem<kTallWaves> s_plan;
   __shared__ __align__(16) union { TallMem<D> unit; JoinMem join; } s;
-  run_units<D, true, kTallWaves>(a, scratch, tickets, s_plan, s.join,
+  run_units<D, kTall, kTallWaves>(a, scratch, tickets, s_plan, s.join,
                                  [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
                                    tall_unit<D>(a, c, u, hk, chunk, to, s.unit);
                                  });
@@ -1132,27 +1193,30 @@ __global__ __launch_bounds__(kTallWaves *kWave, D == 128 ? 2 : 4) void attn_page
 
 template <int D>
 void launch(hipStream_t st, const AttnArgs &a, float *scratch, unsigned *tickets) {
+  const dim3 few(kShortWaves * kWave), many(kTallWaves * kWave);
   if (attention_paged_tall(a.T, a.B, a.G)) {
-    hipLaunchKernelGGL(attn_paged_tall_kernel<D>, dim3(kSlots), dim3(kTallWaves * kWave), 0, st, a,
-                       scratch, tickets);
-    return;
+    hipLaunchKernelGGL(attn_paged_tall_kernel<D>, dim3(kSlots), many, 0, st, a, scratch, tickets);
+  } else if (attention_paged_solo(a.T, a.B, a.G, a.p.Hkv)) {
+    hipLaunchKernelGGL(attn_paged_solo_kernel<D>, dim3(kSlots), few, 0, st, a, scratch, tickets);
+  } else {
+    // as many workgroups as there can be units, up to two a CU
+    const int64_t bound = (int64_t)kSlots +
+        (((int64_t)a.T * a.G + kCols - 1) / kCols + std::min(a.B, a.T)) * a.p.Hkv;
+    hipLaunchKernelGGL(attn_paged_short_kernel<D>, dim3((unsigned)std::min<int64_t>(bound, kSlots)),
+                       few, 0, st, a, scratch, tickets);
   }
-  // as many workgroups as there can be units, up to two a CU
-  const int64_t bound = (int64_t)kSlots +
-      (((int64_t)a.T * a.G + kCols - 1) / kCols + std::min(a.B, a.T)) * a.p.Hkv;
-  hipLaunchKernelGGL(attn_paged_short_kernel<D>, dim3((unsigned)std::min<int64_t>(bound, kSlots)),
-                     dim3(kShortWaves * kWave), 0, st, a, scratch, tickets);
 }
 
 }  // namespace
 
 // Units that share their group.  Short: with room = kSlots - groups, work / chunk +
 // groups of them, kSlots; with room = kShortRoom, tiles / chunk + 1 < 2 tiles / chunk
-// for each group that has several, 2 kShortRoom.  Tall: likewise 2 kSlots.
+// for each group that has several, 2 kShortRoom.  Likewise 2 kSoloSlots of 16 and
+// 2 kSlots of 128 columns, and half as many groups.
 int64_t attention_paged_part_elems(int D) {
-  return std::max((int64_t)kSlots * kCols, (int64_t)2 * kSlots * kTallCols) * (D + 2);
+  return std::max((int64_t)2 * kSoloSlots * kCols, (int64_t)2 * kSlots * kTallCols) * (D + 2);
 }
-int attention_paged_tickets() { return kSlots + 2; }
+int attention_paged_tickets() { return kTickets + 2; }
 
 void launch_attention_paged(hipStream_t st, const float *q, int T, const int8_t *codes,
                             const float *scales, const PagedPool &p, const int32_t *tables,
