@@ -139,8 +139,8 @@ __device__ inline float *out_row(const AttnArgs &a, const Columns &c, int hk, in
 
 // Two floats that a workgroup of another die reads: written through and read past
 // the die's cache.  (A fence in their place would empty the cache for the other
-// workgroups, whose keys and values lie in it: 4 x 1000 rows, 63 us with a fence
-// after the counter, @@ without.)
+// workgroups, whose keys and values lie in it: 4 x 1000 rows of 16 heads over 4 of 64
+// dims in ranges of 10 tiles, 63 us with a fence after the counter, 60 without.)
 __device__ inline float2 get2(const float *p) {
   const uint64_t bits = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED,
                                           __HIP_MEMORY_SCOPE_AGENT);
@@ -168,8 +168,8 @@ __device__ inline void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
 // Units.
 //
 // A unit is a tile of columns of one request and kv head over a range of `chunk`
-// key tiles: 128 columns where the requests have many on average
-// (attn_paged_tall_kernel), else 16 (attn_paged_short_kernel).  The lengths are on
+// key tiles: 128 columns where the requests fill them (attn_paged_tall_kernel), else
+// 16 (attn_paged_short_kernel, and attn_paged_solo_kernel for many of them).  The lengths are on
 // the device, so every workgroup forms the sums over the requests itself and takes
 // its units from them; the ranges are chosen so that the units of a launch fill the
 // chip, whatever the lengths are.  Where a group of columns has several ranges, each
@@ -183,9 +183,17 @@ constexpr int kSlots = 512;              // workgroups that run at once: two a C
 __device__ inline int tall_slots(int D) { return D == 128 ? kSlots / 2 : kSlots; }
 constexpr int kShortRoom = kSlots / 4;   // least slots that are shared out by tiles
 constexpr int kSoloSlots = kSlots * kShortWaves;
-constexpr int kTickets = kSoloSlots;     // counters of groups, then the queue's two
+constexpr int kTickets = kSoloSlots;     // counters of groups, then the queues'
+// Queues of units, of which a workgroup uses the one of its index, and so mostly of
+// its die: takes of one counter are 12 ns apart.  Their counters lie in lines of
+// their own, and behind them the one of the workgroups that have ended.
+constexpr int kQueues = 8, kLine = 32;
 enum { kShort, kSolo, kTall };
-constexpr int kShortMin = 8, kTallMin = 16;   // least tiles of a unit of several
+// Least tiles of a unit of several.  Short: 32 requests of up to 1024 tokens 11.3 us
+// with 4, 10.3 with 8, 10.4 with 16; one of 4000 tokens (8 heads of 128 dims) 14.2,
+// 13.0 and 16.0.  Tall: 4 x 1000 rows 61 us with 4, 53 with 16; 200 rows behind 8000
+// tokens 59 and 48; one prompt of 500 rows 19.2 and 20.5.
+constexpr int kShortMin = 8, kTallMin = 16;
 
 struct Part {                            // a request's share of the work
   int first, n, len;                     // its rows, its tokens
@@ -320,7 +328,12 @@ __device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
                    : groups < kSlots ? max(kShortRoom, kSlots - groups * Hkv)
                                      : kShortRoom;
   const float target = work * (1.f + 1.f / 8192) * Hkv / room;
-  const int chunk = max(KIND == kShort ? kShortMin : kTallMin, (int)fminf(target, 1e6f) + 1);
+  // Few long requests: a range costs its own tiles and the join all the ranges'
+  // shares, so neither is much longer than the other (one request of 100000 tokens
+  // and one head of 64 dims: 30 us in ranges of 8 tiles, 21 in ranges of 29).
+  const int least = KIND == kShort ? max(kShortMin, (int)(0.75f * sqrtf(work / max(groups, 1))))
+                                   : kTallMin;
+  const int chunk = max(least, (int)fminf(target, 1e6f) + 1);
   int mine = 0, shares = 0, shared = 0;      // units, those that share a group, such groups
   for (int b = b0; b < b1; ++b) {
     const Part p = part_at(b);
@@ -1091,20 +1104,22 @@ struct Unit {
   __device__ float *share_of(int range) const { return shares + r.place(u.group, range) * step; }
 };
 
-// Workgroups (solo: waves) take their own unit first, the others from a queue, which
-// the last to end leaves empty.  queue[0]: units taken, queue[1]: who has ended.
-__device__ inline void leave_queue(unsigned *queue, unsigned takers) {
-  if (atomicAdd(queue + 1, 1u) == takers - 1) {
-    atomicExch(queue, 0u);
-    atomicExch(queue + 1, 0u);
-  }
+// Workgroups take the unit of their index first, then units from a queue; the last
+// to end leaves the counters zero.
+__device__ inline unsigned take_unit(unsigned *queues) {
+  const unsigned q = blockIdx.x % kQueues;
+  return gridDim.x + kQueues * atomicAdd(queues + kLine * q, 1u) + q;
+}
+__device__ inline void leave_queues(unsigned *queues) {
+  if (atomicAdd(queues + kLine * kQueues, 1u) == gridDim.x - 1)
+    for (int q = 0; q <= kQueues; ++q) atomicExch(queues + kLine * q, 0u);
 }
 
 template <int D, int KIND, int WAVES, typename Run>
 __device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *tickets,
                                  PlanMem<WAVES> &s, JoinMem &jm, Run run) {
   constexpr bool TALL = KIND == kTall;
-  unsigned *queue = tickets + kTickets;
+  unsigned *queues = tickets + kTickets;
   const int Hkv = a.p.Hkv;
   const Plan plan = make_plan<KIND, WAVES>(a, s);
   const int chunk = __builtin_amdgcn_readfirstlane(plan.chunk);
@@ -1112,7 +1127,7 @@ __device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *ti
   unsigned at = blockIdx.x;
   while (at < units) {
     const Unit<D, TALL> w(a, find_unit<TALL, WAVES>(a, s, chunk, at / Hkv), at % Hkv, chunk, scratch);
-    if (threadIdx.x == 0) s.next = gridDim.x + (units > gridDim.x ? atomicAdd(queue, 1u) : 0u);
+    if (threadIdx.x == 0) s.next = units > gridDim.x ? take_unit(queues) : units;
     run(w.c, w.u, w.hk, chunk, w.u.ranges > 1 ? w.share_of(w.u.range) : nullptr);
     if (w.u.ranges > 1 && last_of(tickets + (int64_t)w.u.ticket * Hkv + w.hk, w.u.ranges, &s.last)) {
       auto share_of = [&](int range) { return w.share_of(range); };
@@ -1131,7 +1146,7 @@ __device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *ti
     at = __builtin_amdgcn_readfirstlane(s.next);
     __syncthreads();                   // the LDS is free
   }
-  if (units > gridDim.x && threadIdx.x == 0) leave_queue(queue, gridDim.x);
+  if (units > gridDim.x && threadIdx.x == 0) leave_queues(queues);
 }
 
 // Units of 16 columns with a wave each, where there are so many of them that four
@@ -1194,16 +1209,12 @@ __global__ __launch_bounds__(kTallWaves *kWave, D == 128 ? 2 : 4) void attn_page
 template <int D>
 void launch(hipStream_t st, const AttnArgs &a, float *scratch, unsigned *tickets) {
   const dim3 few(kShortWaves * kWave), many(kTallWaves * kWave);
-  if (attention_paged_tall(a.T, a.B, a.G)) {
+  if (attention_paged_tall(a.T, a.B, a.G, a.p.Hkv)) {
     hipLaunchKernelGGL(attn_paged_tall_kernel<D>, dim3(kSlots), many, 0, st, a, scratch, tickets);
   } else if (attention_paged_solo(a.T, a.B, a.G, a.p.Hkv)) {
     hipLaunchKernelGGL(attn_paged_solo_kernel<D>, dim3(kSlots), few, 0, st, a, scratch, tickets);
   } else {
-    // as many workgroups as there can be units, up to two a CU
-    const int64_t bound = (int64_t)kSlots +
-        (((int64_t)a.T * a.G + kCols - 1) / kCols + std::min(a.B, a.T)) * a.p.Hkv;
-    hipLaunchKernelGGL(attn_paged_short_kernel<D>, dim3((unsigned)std::min<int64_t>(bound, kSlots)),
-                       few, 0, st, a, scratch, tickets);
+    hipLaunchKernelGGL(attn_paged_short_kernel<D>, dim3(kSlots), few, 0, st, a, scratch, tickets);
   }
 }
 
@@ -1216,7 +1227,7 @@ void launch(hipStream_t st, const AttnArgs &a, float *scratch, unsigned *tickets
 int64_t attention_paged_part_elems(int D) {
   return std::max((int64_t)2 * kSoloSlots * kCols, (int64_t)2 * kSlots * kTallCols) * (D + 2);
 }
-int attention_paged_tickets() { return kTickets + 2; }
+int attention_paged_tickets() { return kTickets + kLine * kQueues + 1; }
 
 void launch_attention_paged(hipStream_t st, const float *q, int T, const int8_t *codes,
                             const float *scales, const PagedPool &p, const int32_t *tables,
