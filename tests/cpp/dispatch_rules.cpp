@@ -16,4 +16,10 @@ int sum_short_shape(long long n_out, long long n_red, int along_r) {
 int matmul_short_shape(long long M, long long N, long long K) {
   return nnhip::matmul_short_shape(M, N, K);
 }
+int attention_paged_tall(int T, int B, int G, int Hkv) {
+  return nnhip::attention_paged_tall(T, B, G, Hkv);
+}
+int attention_paged_solo(int T, int B, int G, int Hkv) {
+  return nnhip::attention_paged_solo(T, B, G, Hkv);
+}
 }
