@@ -110,7 +110,15 @@ struct AttnArgs {
 // block, and are masked; a block outside the pool is read as block 0, with scales
 // that make what sees it NaN, as a scale that is no number does.
 constexpr int kHeld = 16;
-struct Held { int blk; float ks, vs, lvs; };   // lvs: log2(vs)
+struct Held {
+  uint32_t head;                                 // index of the block's k among all heads
+  float ks, vs, lvs;                             // lvs: log2(vs)
+};
+// The first code of a head.
+template <int D>
+__device__ inline const int8_t *head_at(const AttnArgs &a, uint32_t head) {
+  return a.codes + ((uint64_t)head << (a.p.lbs + (D == 128 ? 7 : D == 64 ? 6 : 5)));
+}
 __device__ inline Held held_tiles(const AttnArgs &a, const int32_t *table, int tile, int step, int len,
                                   int hk) {
   const int lane = threadIdx.x & 63;
@@ -118,9 +126,9 @@ __device__ inline Held held_tiles(const AttnArgs &a, const int32_t *table, int t
   const int blk = table[min(tok, len - 1) >> a.p.lbs];
   const bool bad = !block_ok(blk, a.p.blocks);
   Held r;
-  r.blk = bad ? 0 : blk;
-  r.ks = scale_ok(a.scales[scale_offset(a.p, r.blk, 0, hk)], bad);
-  r.vs = scale_ok(a.scales[scale_offset(a.p, r.blk, 1, hk)], bad);
+  r.head = (uint32_t)scale_offset(a.p, bad ? 0 : blk, 0, hk);
+  r.ks = scale_ok(a.scales[r.head], bad);
+  r.vs = scale_ok(a.scales[r.head + a.p.Hkv], bad);
   if (r.vs != r.vs) r.ks = r.vs;
   r.lvs = __builtin_amdgcn_logf(r.vs);
   return r;
@@ -709,11 +717,10 @@ __device__ inline void wave_join(const AttnArgs &a, const Columns &c, int hk, in
 }
 
 template <int D>
-__device__ inline void load_k(const AttnArgs &a, int blk, int off, int hk, int lane,
+__device__ inline void load_k(const AttnArgs &a, uint32_t head, int off, int lane,
                               uint32_t (&r)[4][D / 16]) {
   const int m = lane & 15, g = lane >> 4;
-  const int8_t *src = a.codes + head_offset(a.p, blk, 0, hk) +
-                      (int64_t)(off + (m & 3)) * D + g * (D == 32 ? 8 : 16);
+  const int8_t *src = head_at<D>(a, head) + (off + (m & 3)) * D + g * (D == 32 ? 8 : 16);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if constexpr (D == 32) {
@@ -730,10 +737,9 @@ __device__ inline void load_k(const AttnArgs &a, int blk, int off, int hk, int l
 }
 
 template <int D>
-__device__ inline void load_v(const AttnArgs &a, int blk, int off, int hk, int lane,
+__device__ inline void load_v(const AttnArgs &a, uint32_t head, int off, int lane,
                               uint32_t (&r)[D / 16][4]) {
-  const int8_t *src =
-      a.codes + head_offset(a.p, blk, 1, hk) + off + ((lane & 15) << a.p.lbs);
+  const int8_t *src = head_at<D>(a, head + a.p.Hkv) + off + ((lane & 15) << a.p.lbs);
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) {
     const uint4 v = *reinterpret_cast<const uint4 *>(src + (d << (4 + a.p.lbs)));
@@ -783,9 +789,10 @@ __device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, 
   // places of the tile's tokens 16 m4 (k) and 16 g (v, scales) in their blocks
   auto place = [&](int tile, int sub) { return (tile * kKeys + 16 * sub) & (a.p.bs - 1); };
   Held held = held_tiles(a, c.table, t, STEP, c.len, hk);
-  int at = 0, vblk = __shfl(held.blk, g, kWave);
-  load_k<D>(a, __shfl(held.blk, m4, kWave), place(t, m4), hk, lane, kr);
-  load_v<D>(a, vblk, place(t, g), hk, lane, vr);
+  int at = 0;
+  auto head = [&](int sub) { return (uint32_t)__shfl((int)held.head, 4 * at + sub, kWave); };
+  load_k<D>(a, head(m4), place(t, m4), lane, kr);
+  load_v<D>(a, head(g), place(t, g), lane, vr);
   const Query<D> q = load_query<D>(a, c, hk, lane & 15, D == 32 ? 32 : 64, D == 32 ? 8 : 16);
   for (; t + STEP < end; t += STEP) {
     const float ks = __shfl(held.ks, 4 * at + g, kWave), vs = __shfl(held.vs, 4 * at + g, kWave);
@@ -794,11 +801,10 @@ __device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, 
       held = held_tiles(a, c.table, t + STEP, STEP, c.len, hk);
       at = 0;
     }
-    const int kblk = __shfl(held.blk, 4 * at + m4, kWave);
-    vblk = __shfl(held.blk, 4 * at + g, kWave);
+    const uint32_t k_head = head(m4), v_head = head(g);
     float4_t acc[4] = {};
     short_scores<D>(kr, q, acc);
-    load_k<D>(a, kblk, place(t + STEP, m4), hk, lane, kr);
+    load_k<D>(a, k_head, place(t + STEP, m4), lane, kr);
     half8_t hi[2], lo[2];
     if ((t + 1) * kKeys <= least)
       softmax_tile<D, false>(st, acc, ks, vs, lvs, q.mul, 16, hi, lo);
@@ -806,7 +812,7 @@ __device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, 
       softmax_tile<D, true>(st, acc, ks, vs, lvs, q.mul, min(q.see - t * kKeys, kKeys) - 16 * g, hi,
                             lo);
     short_sums<D>(vr, hi, lo, st);
-    load_v<D>(a, vblk, place(t + STEP, g), hk, lane, vr);
+    load_v<D>(a, v_head, place(t + STEP, g), lane, vr);
   }
   // the last tile on its own: a condition on the loads within the loop would have
   // them all waited for
@@ -894,52 +900,71 @@ __device__ inline float lane_of(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
-// The codes of a tile that a thread brings: an eighth of a token's dims of k, and,
-// of v, 16 tokens of a dim (the first 4 D threads).
+// The codes of a tile that a thread brings, 16 of them: of k 16 dims of a token, of v
+// 16 tokens of a dim.  Waves bring either (k: the waves behind v's), or, for 128 dims,
+// both.  Every address is a head's and one of 32 bits.
 template <int D>
-struct TallLoad { uint32_t k[D / 32], v[4]; };
+struct TallLoad { uint4 k, v; };                 // D < 128: v alone, for both
 template <int D>
-__device__ inline void tall_load(const AttnArgs &a, int hk, int kblk, int koff, int vblk, int voff,
+constexpr int tall_first() { return D == 128 ? 0 : 4 * D; }  // k's first thread
+__device__ inline int tall_thread() { return thread_here() & (kTallWaves * kWave - 1); }
+template <int D>
+__device__ inline void tall_load(const AttnArgs &a, const Held &h, int at, int tok, int wave,
                                  TallLoad<D> &r) {
-  const int tid = thread_here();
-  const int8_t *kp = a.codes + head_offset(a.p, kblk, 0, hk) +
-                     (int64_t)(koff + ((tid >> 3) & 15)) * D + (tid & 7) * (D / 8);
-  if constexpr (D == 32) {
-    r.k[0] = *reinterpret_cast<const uint32_t *>(kp);
-  } else if constexpr (D == 64) {
-    const uint2 x = *reinterpret_cast<const uint2 *>(kp);
-    r.k[0] = x.x; r.k[1] = x.y;
-  } else {
-    const uint4 x = *reinterpret_cast<const uint4 *>(kp);
-    r.k[0] = x.x; r.k[1] = x.y; r.k[2] = x.z; r.k[3] = x.w;
-  }
-  if (tid < 4 * D) {
-    const uint4 x = *reinterpret_cast<const uint4 *>(
-        a.codes + head_offset(a.p, vblk, 1, hk) + voff + ((tid >> 2) << a.p.lbs));
-    r.v[0] = x.x; r.v[1] = x.y; r.v[2] = x.z; r.v[3] = x.w;
+  const int m = a.p.bs - 1;
+  auto load = [](const int8_t *p) { return *reinterpret_cast<const uint4 *>(p); };
+  auto head = [&](int sub) { return (uint32_t)__shfl((int)h.head, 4 * at + sub, kWave); };
+  auto load_k = [&] {
+    const int id = tall_thread() - tall_first<D>();
+    if constexpr (D == 32) {
+      const int sub = (id >> 5) & 3;
+      return load(head_at<D>(a, head(sub)) + (((tok + 16 * sub) & m) * D + (id & (D - 1)) * 16));
+    } else {
+      const int sub = (wave - tall_first<D>() / kWave) / (D / kWave);
+      const uint32_t k = __builtin_amdgcn_readlane(h.head, 4 * at + sub);
+      return load(head_at<D>(a, k) + ((tok + 16 * sub) & m) * D + (id & (D - 1)) * 16);
+    }
+  };
+  auto load_v = [&] {
+    const int id = tall_thread(), sub = id & 3;
+    return load(head_at<D>(a, head(sub) + a.p.Hkv) +
+                (((tok + 16 * sub) & m) + ((id >> 2) << a.p.lbs)));
+  };
+  if constexpr (D == 128) {
+    r.k = load_k();
+    r.v = load_v();
+  } else if (wave < 4 * D / kWave) {
+    r.v = load_v();
+  } else if (wave < 8 * D / kWave) {
+    r.v = load_k();
   }
 }
 template <int D>
-__device__ inline void tall_store(TallMem<D> &s, int buf, const TallLoad<D> &r) {
-  const int tid = thread_here(), token = tid >> 3, c8 = tid & 7;
-  if constexpr (D == 32) {
-    const half8_t x = codes8(r.k[0], 0);
-    reinterpret_cast<uint2 *>(s.k[buf][token])[c8] = make_uint2(as_u4(x).x, as_u4(x).y);
-  } else {
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i)
-      s.k[buf][token][D / 64 * c8 + i] = as_u4(codes8(r.k[2 * i], r.k[2 * i + 1]));
-  }
-  if (tid < 4 * D) {
+__device__ inline void tall_store(TallMem<D> &s, int buf, int wave, const TallLoad<D> &r) {
+  auto store_k = [&](const uint4 &x) {
+    const int id = tall_thread() - tall_first<D>();
+    uint4 *row = &s.k[buf][0][0] + __umul24(id / (D / 16), D / 8 + 1) + 2 * (id & (D / 16 - 1));
+    row[0] = as_u4(codes8(x.x, x.y));
+    row[1] = as_u4(codes8(x.z, x.w));
+  };
+  auto store_v = [&](const uint4 &x) {
     // block b of the tile: tokens 4 g .. of it, at half b % 2 of piece 4 (b / 2) + g
-    const int b = tid & 3;
-    uint2 *row = reinterpret_cast<uint2 *>(s.v[buf][tid >> 2]) + 8 * (b >> 1) + (b & 1);
-#pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      const uint4 x = as_u4(codes8(r.v[g], r.v[g + 1]));
-      row[2 * g] = make_uint2(x.x, x.y);
-      row[2 * g + 2] = make_uint2(x.z, x.w);
-    }
+    const int id = tall_thread(), b = id & 3;
+    uint2 *row = reinterpret_cast<uint2 *>(&s.v[buf][0][0]) + __umul24(id >> 2, 18) + 8 * (b >> 1) +
+                 (b & 1);
+    const uint4 lo = as_u4(codes8(x.x, x.y)), hi = as_u4(codes8(x.z, x.w));
+    row[0] = make_uint2(lo.x, lo.y);
+    row[2] = make_uint2(lo.z, lo.w);
+    row[4] = make_uint2(hi.x, hi.y);
+    row[6] = make_uint2(hi.z, hi.w);
+  };
+  if constexpr (D == 128) {
+    store_k(r.k);
+    store_v(r.v);
+  } else if (wave < 4 * D / kWave) {
+    store_v(r.v);
+  } else if (wave < 8 * D / kWave) {
+    store_k(r.v);
   }
 }
 
@@ -1050,19 +1075,14 @@ __device__ inline void tall_unit(const AttnArgs &a, const Columns &c, const Pick
   State<D> st;
   if (start < end) {
     TallLoad<D> r;
-    const int kt = 16 * (wave >> 1), vt = 16 * (tid & 3);   // the thread's tokens of a tile
-    auto load = [&](const Held &h, int at, int tile) {
-      const int tok = tile * kKeys, m = a.p.bs - 1;
-      tall_load<D>(a, hk, __builtin_amdgcn_readlane(h.blk, 4 * at + (wave >> 1)), (tok + kt) & m,
-                   __shfl(h.blk, 4 * at + (tid & 3), kWave), (tok + vt) & m, r);
-    };
     Held held = held_tiles(a, c.table, start, 1, c.len, hk);
-    int at = 0;
-    load(held, 0, start);
+    int at = 0, t = start;
+    tall_load<D>(a, held, 0, start * kKeys, wave, r);
     const Query<D> q = load_query<D>(a, c, hk, col, 32, 8);
-    tall_store<D>(s, 0, r);
+    tall_store<D>(s, 0, wave, r);
     __syncthreads();
-    for (int t = start; t < end; ++t) {
+    // a tile, while the next one's codes are on their way
+    auto step = [&](auto tile) {
       const int buf = (t - start) & 1;
       const Scales sc = scales_of(held, at);
       if (t + 1 < end) {
@@ -1070,15 +1090,21 @@ __device__ inline void tall_unit(const AttnArgs &a, const Columns &c, const Pick
           held = held_tiles(a, c.table, t + 1, 1, c.len, hk);
           at = 0;
         }
-        load(held, at, t + 1);
+        tall_load<D>(a, held, at, (t + 1) * kKeys, wave, r);
       }
-      if ((t + 1) * kKeys <= least)
-        tall_tile<D, false>(s, buf, sc, q, st, kKeys);
-      else if (t * kKeys < most)
-        tall_tile<D, true>(s, buf, sc, q, st, min(q.see - t * kKeys, kKeys) - 4 * g);
-      if (t + 1 < end) tall_store<D>(s, buf ^ 1, r);
+      tile(buf, sc);
+      if (t + 1 < end) tall_store<D>(s, buf ^ 1, wave, r);
       __syncthreads();
-    }
+    };
+    // tiles that the wave's columns see whole, then the others: two loops, whose sums
+    // stay in the registers that they are in
+    for (const int whole = min(end, least / kKeys); t < whole; ++t)
+      step([&](int buf, const Scales &sc) { tall_tile<D, false>(s, buf, sc, q, st, kKeys); });
+    for (; t < end; ++t)
+      step([&](int buf, const Scales &sc) {
+        if (t * kKeys < most)
+          tall_tile<D, true>(s, buf, sc, q, st, min(q.see - t * kKeys, kKeys) - 4 * g);
+      });
   }
   if (any) wave_end<D>(a, c, hk, col, cols, u.ranges, share_at, wave, kTallCols, st);
 }
