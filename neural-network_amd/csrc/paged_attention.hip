@@ -199,8 +199,8 @@ constexpr int kQueues = 8, kLine = 32;
 enum { kShort, kSolo, kTall };
 // Least tiles of a unit of several.  Short: 32 requests of up to 1024 tokens 11.3 us
 // with 4, 10.3 with 8, 10.4 with 16; one of 4000 tokens (8 heads of 128 dims) 14.2,
-// 13.0 and 16.0.  Tall: 4 x 1000 rows 61 us with 4, 53 with 16; 200 rows behind 8000
-// tokens 59 and 48; one prompt of 500 rows 19.2 and 20.5.
+// 13.0 and 16.0.  Tall: 4 x 1000 rows of 64 dims 55 us with 6 to 11, 51 with 16; 800
+// rows 27 with 8, 29 with 16.
 constexpr int kShortMin = 8, kTallMin = 16;
 
 struct Part {                            // a request's share of the work
@@ -1012,14 +1012,15 @@ __device__ inline void tall_tile(const TallMem<D> &s, int buf, const Scales &sc,
     xm = fmaxf(xm, x);
     am = fmaxf(am, x + sc.lvs[t]);
   }
-  // unconditional: a branch around the sums would have them copied
   const float m = fmaxf(st.m, ceilf(max_groups(xm)));
   st.l *= share(st.m, m);
   st.m = m;
   const float E = fmaxf(st.E, ceilf(max_groups(am)));
-  const float f = __builtin_amdgcn_exp2f(st.E - E);
+  if (__any(st.E != E)) {              // seldom, after the first tiles
+    const float f = __builtin_amdgcn_exp2f(st.E - E);
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) st.o[i] *= f;
+    for (int i = 0; i < D / 16; ++i) st.o[i] *= f;
+  }
   st.E = E;
   const float base = m == -INFINITY ? 0.f : m;
   const int shift = (int)(base - E) + 15;
