@@ -389,7 +389,8 @@ int nnhip_spec_accept(nnhip_ctx *ctx, const float *tlogits,
  * scale for each block and head where KVCache(true) has one for each row.
  *
  * Pool: num_blocks blocks of block_size tokens (16, 32, 64 or 128; at most
- * 2^31 - 1 slots in all; a table row names at most 2^30 tokens).
+ * 2^31 - 1 slots and as many heads of blocks in all; a table row names at most
+ * 2^30 tokens).
  *   codes  [num_blocks][2][Hkv][block_size * D] int8, aligned to 16 bytes:
  *          k (index 0) as [block_size][D], v (index 1) as [D][block_size]
  *   scales [num_blocks][2][Hkv] fp32, not negative; a cached value is code *
@@ -429,8 +430,8 @@ int nnhip_block_tables(nnhip_ctx *ctx, int B, const int32_t *cached,
 /* RoPE on q and k of qkv [T][q: H heads | k: Hkv | v: Hkv] rows of D, pairs
  * (2j, 2j + 1) turned by cos_t / sin_t [n_pos][D / 2] at pos[t] (both NULL: the
  * reference's angles, tensor.cpp:1141-1173), q_out [T][H * D], then k and v
- * into slots[t] of the pool.  The rows of one block lie within block_size rows
- * of one another, in any order (where several name a slot, the last counts).
+ * into slots[t] of the pool.  All rows of one block lie within some block_size
+ * rows on end, in any order (where several name a slot, the last counts).
  * The scale of a (block, k or v, head) is the smallest power of two 2^e, e >=
  * -126, with max|x| <= 127 * 2^e over the rows it is given (0 when they are all
  * 0), codes are x / scale rounded to the nearest, ties to even.  A call that

@@ -207,9 +207,8 @@ __global__ __launch_bounds__(THREADS) void block_tables_kernel(
 // threads share it.  A decode step has a leader a row, of one token: a wave takes
 // one after another.  The first quads that a thread has looked at for the scale stay
 // in registers until their codes are stored (more of them cost workgroups a unit:
-// two 22 us, four 27, one 20, where the rest is read from L2 again), and v, whose
-// products are exact, is done in 32 bits.  The queries are rotated by workgroups
-// behind those.
+// two 22 us, four 27, one 20, where the rest is read from L2 again).  The queries are
+// rotated by workgroups behind those.
 //
 // 9 prompts of up to 1000 tokens (7835 rows, 16 heads over 4 of 64 dims): 20 us,
 // 4.6 TB/s; bound by memory at that size.  A step of 27 requests: 5 us, latency.
@@ -285,7 +284,6 @@ __device__ inline int pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
 __device__ inline uint32_t code(double x, double inv) {
   return (uint32_t)__double_as_longlong(fma(x, inv, 0x1.8p52));
 }
-__device__ inline uint32_t code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 0x1.8p23f)); }
 
 // Larger of m and |x|, as bits without the sign: in the order of the values, and
 // infinities and NaN from 0xff000000.
@@ -406,7 +404,6 @@ __device__ void append_block(const AppendRows &a, const PagedPool &p, const int 
     kd[i] = ks.none ? 0 : pack4(code(x[0], ks.inv), code(x[1], ks.inv), code(x[2], ks.inv),
                                 code(x[3], ks.inv));
   };
-  const float v_inv = (float)vs.inv;
   auto v_store = [&](const float4 &q, int word, int i) {
     if (i >= v_end) return;
     const int4 r = v_rows(i);
@@ -418,8 +415,8 @@ __device__ void append_block(const AppendRows &a, const PagedPool &p, const int 
     } else if ((r.x & r.y & r.z & r.w) < 0) {
       return;
     }
-    const int now = vs.none ? 0 : pack4(code(q.x, v_inv), code(q.y, v_inv), code(q.z, v_inv),
-                                        code(q.w, v_inv));
+    const int now = vs.none ? 0 : pack4(code(q.x, vs.inv), code(q.y, vs.inv), code(q.z, vs.inv),
+                                        code(q.w, vs.inv));
     const int m = (r.x < 0 ? 0 : 255) | (r.y < 0 ? 0 : 255 << 8) | (r.z < 0 ? 0 : 255 << 16) |
                   (r.w < 0 ? 0 : 255 << 24);
     vd[v_dim(i) * (p.bs / 4) + w] = (now & m) | (word & ~m);

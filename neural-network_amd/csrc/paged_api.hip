@@ -32,6 +32,8 @@ nnhip::PagedPool pool_of(int block_size, int num_blocks, int Hkv, int D, const v
   REQ(num_blocks > 0 && (int64_t)num_blocks * block_size <= INT32_MAX,
       std::string(what) + ": num_blocks must be positive, with at most 2^31 - 1 token slots");
   REQ(Hkv > 0 && Hkv <= 4096, std::string(what) + ": Hkv out of range");
+  REQ((int64_t)num_blocks * 2 * Hkv <= INT32_MAX,
+      std::string(what) + ": num_blocks * Hkv must be below 2^30");
   NNHIP_REQUIRE(D == 32 || D == 64 || D == 128, nnhip::kErrUnsupported,
                 std::string(what) + ": head dim must be 32, 64 or 128");
   REQ(aligned(codes, 16) && aligned(scales, 4), std::string(what) + ": codes must be aligned to 16 bytes");

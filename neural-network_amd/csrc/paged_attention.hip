@@ -177,12 +177,12 @@ __device__ inline void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
 //
 // A unit is a tile of columns of one request and kv head over a range of `chunk`
 // key tiles: 128 columns where the requests fill them (attn_paged_tall_kernel), else
-// 16 (attn_paged_short_kernel, and attn_paged_solo_kernel for many of them).  The lengths are on
-// the device, so every workgroup forms the sums over the requests itself and takes
-// its units from them; the ranges are chosen so that the units of a launch fill the
-// chip, whatever the lengths are.  Where a group of columns has several ranges, each
-// unit leaves its state in the scratch, and the last to arrive (a counter a group,
-// left zero) joins them.
+// 16 (attn_paged_short_kernel, and attn_paged_solo_kernel for many of them).  The
+// lengths are on the device, so every workgroup forms the sums over the requests
+// itself and takes its units from them; the ranges are chosen so that the units of a
+// launch fill the chip, whatever the lengths are.  Where a group of columns has
+// several ranges, each unit leaves its state in the scratch, and the last to arrive
+// (a counter a group, left zero) joins them, in their order.
 constexpr int kShortWaves = 4, kTallWaves = 8;
 constexpr int kTallCols = kCols * kTallWaves;
 constexpr int kSlots = 512;              // workgroups that run at once: two a CU
@@ -196,6 +196,7 @@ constexpr int kTickets = kSoloSlots;     // counters of groups, then the queues'
 // its die: takes of one counter are 12 ns apart.  Their counters lie in lines of
 // their own, and behind them the one of the workgroups that have ended.
 constexpr int kQueues = 8, kLine = 32;
+static_assert(kSlots % kQueues == 0, "the queues share out all units");
 enum { kShort, kSolo, kTall };
 // Least tiles of a unit of several.  Short: 32 requests of up to 1024 tokens 11.3 us
 // with 4, 10.3 with 8, 10.4 with 16; one of 4000 tokens (8 heads of 128 dims) 14.2,

@@ -313,6 +313,48 @@ def test_append_of_other_numbers_of_heads(ctx, H, Hkv):
     c.assert_same()
 
 
+@pytest.mark.parametrize("bs", [16, 32])
+@pytest.mark.parametrize("lead", [0, 1, 3, 14, 15, 17])
+def test_append_of_blocks_that_share_rows_on_end(ctx, bs, lead):
+    """Two blocks by turns over bs rows, wherever these begin; among many others."""
+    rng = np.random.default_rng(lead)
+    for n, Hkv in ((70, 2), (1600, 8)):
+        blocks = n // bs + 4
+        c = Cache(ctx, blocks, Hkv, 64, bs, rng)
+        ids = rng.permutation(blocks)
+        slots = np.full(n, -1)
+        for i, at in enumerate(range(lead, n - bs + 1, bs)):
+            pair = ids[2 * (i // 2):2 * (i // 2) + 2] if i % 2 == 0 else None
+            if pair is None:
+                continue
+            off = rng.permutation(bs)
+            slots[at:at + bs] = pair[np.arange(bs) % 2] * bs + off
+        pos = rng.integers(0, 60, n)
+        qkv = rng.standard_normal((n, 3 * Hkv * 64)).astype(np.float32)
+        cos, sin = angles(60, 64)
+        q_close(*c.append(qkv, pos, slots, Hkv, cos, sin))
+        c.assert_same()
+
+
+@pytest.mark.parametrize("n", [1, 9])
+def test_append_behind_any_scale(ctx, n):
+    """Blocks whose scale is no power of two, or below the smallest that a call
+    sets: it is kept while the new values fit."""
+    rng = np.random.default_rng(n)
+    bs, Hkv, D = 16, 4, 64
+    c = Cache(ctx, 40, Hkv, D, bs, rng)
+    c.scales[:] = rng.uniform(0.05, 0.3, c.scales.shape).astype(np.float32)
+    c.scales[5:9] = 2.0 ** -140
+    c.scales[9:12] = 0
+    c.ds.upload(c.scales)
+    pos, slots = rows_of([([b], 3, n) for b in range(40)], bs)
+    qkv = rng.standard_normal((len(pos), 3 * Hkv * D)).astype(np.float32)
+    qkv[(slots // bs == 5) | (slots // bs == 9)] = 0
+    cos, sin = angles(20, D)
+    q_close(*c.append(qkv, pos, slots, Hkv, cos, sin))
+    c.assert_same()
+
+
 @pytest.mark.parametrize("where", [0, 7, 15])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf, 3e38])
 def test_append_of_one_value_among_many(ctx, where, value):

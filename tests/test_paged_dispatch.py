@@ -1,9 +1,12 @@
 """Which kernel paged attention runs on (csrc/dispatch.hpp), asked on the CPU: most
 shapes below were timed with the kernels on an MI355X, and the rule takes the
 fastest one for most contexts (the lengths are on the device)."""
+import os
+
 import pytest
 
-from gpu_util import dispatch_rules
+from gpu_util import dispatch_rules, nnhip
+from test_paged import OPS
 
 
 @pytest.fixture(scope="module")
@@ -26,3 +29,18 @@ def test_paged_attention(rules, T, B, G, Hkv, want):
     got = "tall" if rules.attention_paged_tall(T, B, G, Hkv) else \
         "solo" if rules.attention_paged_solo(T, B, G, Hkv) else "short"
     assert got == want
+
+
+@pytest.mark.skipif(not os.path.exists(nnhip.LIB_PATH), reason="libnnhip.so not built")
+@pytest.mark.parametrize("op", ["nnhip_rope_kv_append_paged_q8", "nnhip_attention_paged_q8",
+                                "nnhip_kv_read_paged_q8"])
+def test_a_pool_of_more_heads_than_are_counted_is_refused(op):
+    good = dict(OPS[op], num_blocks=2 ** 20, Hkv=1024)
+    if "H" in good:
+        good["H"] = 1024
+    with pytest.raises(nnhip.NNHipError, match="num_blocks") as e:
+        nnhip.call(op, *good.values())
+    assert e.value.code == nnhip.EARG
+    good["num_blocks"] = 2 ** 20 - 1              # as many as there may be: the next check
+    with pytest.raises(nnhip.NNHipError, match="NULL"):
+        nnhip.call(op, *good.values())
