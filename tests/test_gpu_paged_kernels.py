@@ -264,6 +264,36 @@ def test_a_row_that_is_no_number(ctx, rules, kind, value):
     assert np.isnan(got[head]).all() and np.array_equal(got[~head], first[~head])
 
 
+@pytest.mark.parametrize("kind,H,B", [("tall", 128, 1), ("solo", 8, 200)])
+def test_codes_beyond_32_bits(ctx, rules, kind, H, B):
+    """Blocks past 2^32 bytes of codes: what the same blocks give at the start."""
+    D, bs, Hkv, T = 128, 128, 8, 265 if kind == "tall" else B
+    blocks = 2 ** 32 // (2 * Hkv * bs * D) + 40
+    assert kernel(rules, T, B, H, Hkv) == kind
+    rng = np.random.default_rng(27)
+    codes = ctx.array(shape=(blocks, 2, Hkv, bs * D), dtype=np.int8)
+    scales = ctx.array(shape=(blocks, 2, Hkv))
+    n = 1100
+    qkv = ctx.array(rng.standard_normal((n, 3 * Hkv * D)).astype(np.float32))
+    q = ctx.array(rng.standard_normal((T, H * D)).astype(np.float32))
+    start = ctx.array(i32([0, T] if kind == "tall" else range(B + 1)))
+    lens = ctx.array(i32([n] * B))
+    got = []
+    for ids in (np.arange(9), blocks - 1 - 3 * np.arange(9)):
+        pos, slots = rows_of([(ids, 0, n)], bs)
+        p, s = ctx.array(i32(pos)), ctx.array(i32(slots))
+        t = ctx.array(i32(np.tile(ids, (B, 1))))
+        turned, out = (ctx.array(np.zeros(sh, np.float32)) for sh in ((n, Hkv * D), (T, H * D)))
+        nnhip.call("nnhip_rope_kv_append_paged_q8", ctx.h, qkv.p, n, Hkv, Hkv, D, p.p, s.p, None,
+                   None, n, turned.p, codes.p, scales.p, bs, blocks)
+        nnhip.call("nnhip_attention_paged_q8", ctx.h, q.p, T, codes.p, scales.p, bs, blocks, t.p, 9,
+                   start.p, lens.p, B, H, Hkv, D, out.p)
+        got.append((turned.numpy(), out.numpy()))
+    for a, b in zip(*got):
+        assert np.abs(a).max() > 0 and np.array_equal(a, b)
+    codes.free()
+
+
 # ------------------------------------------------------------------ append ----
 @pytest.mark.parametrize("D,bs,Hkv,n", [(64, 16, 16, 520), (128, 64, 8, 1000), (32, 128, 16, 700)])
 def test_append_of_many_single_tokens(ctx, D, bs, Hkv, n):
