@@ -211,7 +211,7 @@ __global__ __launch_bounds__(THREADS) void block_tables_kernel(
 // rotated by workgroups behind those.
 //
 // 9 prompts of up to 1000 tokens (7835 rows, 16 heads over 4 of 64 dims): 20 us,
-// 4.6 TB/s; bound by memory at that size.  A step of 27 requests: 5 us, latency.
+// 4.3 TB/s; bound by memory at that size.  A step of 27 requests: 5 us, latency.
 
 struct AppendRows {
   const float *qkv;
