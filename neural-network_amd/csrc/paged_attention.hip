@@ -293,7 +293,10 @@ struct PlanMem {
   int next, last;
 };
 
-struct Plan { int units, chunk; };         // of a kv head; tiles of a unit
+struct Plan {
+  int units, chunk;                        // of a kv head; tiles of a unit
+  float work;                              // tiles of all groups of a kv head
+};
 template <int KIND, int WAVES>
 __device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
   constexpr int kThreads = WAVES * kWave;
@@ -372,7 +375,7 @@ __device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
   s.slot[tid] = sat - shares;
   s.ticket[tid] = gat - shared;
   __syncthreads();
-  return Plan{all, chunk};
+  return Plan{all, chunk, work};
 }
 
 // Unit `item` (of a kv head), the same for the whole wave.
@@ -547,7 +550,7 @@ __device__ inline void join_few(const AttnArgs &a, const Columns &c, int hk, int
 // 4 t + i, all of one block; the left operand of the products with v holds dim
 // 16 d + r, the 16 tokens of block g.
 //
-// 4 requests of up to 131072 tokens, 32 heads on 8 of 128 dims: 109 us, 5.1 TB/s, bound
+// 4 requests of up to 131072 tokens, 32 heads on 8 of 128 dims: 105 us, 5.3 TB/s, bound
 // by memory.  2 chunks of 500 rows beside 31 requests that decode, 16 heads on 4 of
 // 128: 62 us, bound by VALU, two fifths of it the codes to halves, which every wave
 // forms for its own 16 columns.  32 requests of up to 1024 tokens: 9.5 us, latency.
@@ -722,7 +725,17 @@ __device__ inline void wave_join(const AttnArgs &a, const Columns &c, int hk, in
   if (col < cols) wave_out<D>(a, c, hk, col, g, o, L);
 }
 
-template <int D>
+// 16 codes; ONCE: which no other unit reads, and which are not kept in the caches.
+template <bool ONCE>
+__device__ inline uint4 load16(const int8_t *p) {
+  if constexpr (ONCE) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const u4 x = __builtin_nontemporal_load(reinterpret_cast<const u4 *>(p));
+    return make_uint4(x.x, x.y, x.z, x.w);
+  }
+  return *reinterpret_cast<const uint4 *>(p);
+}
+template <int D, bool ONCE>
 __device__ inline void load_k(const AttnArgs &a, uint32_t head, int off, int lane,
                               uint32_t (&r)[4][D / 16]) {
   const int m = lane & 15, g = lane >> 4;
@@ -735,20 +748,20 @@ __device__ inline void load_k(const AttnArgs &a, uint32_t head, int off, int lan
     } else {
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(src + 4 * t * D + 64 * i);
+        const uint4 v = load16<ONCE>(src + 4 * t * D + 64 * i);
         r[t][4 * i] = v.x; r[t][4 * i + 1] = v.y; r[t][4 * i + 2] = v.z; r[t][4 * i + 3] = v.w;
       }
     }
   }
 }
 
-template <int D>
+template <int D, bool ONCE>
 __device__ inline void load_v(const AttnArgs &a, uint32_t head, int off, int lane,
                               uint32_t (&r)[D / 16][4]) {
   const int8_t *src = head_at<D>(a, head + a.p.Hkv) + off + ((lane & 15) << a.p.lbs);
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(src + (d << (4 + a.p.lbs)));
+    const uint4 v = load16<ONCE>(src + (d << (4 + a.p.lbs)));
     r[d][0] = v.x; r[d][1] = v.y; r[d][2] = v.z; r[d][3] = v.w;
   }
 }
@@ -784,7 +797,7 @@ __device__ inline void short_sums(const uint32_t (&vr)[D / 16][4], const half8_t
 }
 
 // The state of a wave after key tiles t, t + STEP, .. below `end`, of 16 columns.
-template <int D, int STEP>
+template <int D, int STEP, bool ONCE>
 __device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, int t, int end,
                                    State<D> &st) {
   const int lane = thread_here() & 63, g = lane >> 4, m4 = (lane & 15) >> 2;
@@ -797,8 +810,8 @@ __device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, 
   Held held = held_tiles(a, c.table, t, STEP, c.len, hk);
   int at = 0;
   auto head = [&](int sub) { return (uint32_t)__shfl((int)held.head, 4 * at + sub, kWave); };
-  load_k<D>(a, head(m4), place(t, m4), lane, kr);
-  load_v<D>(a, head(g), place(t, g), lane, vr);
+  load_k<D, ONCE>(a, head(m4), place(t, m4), lane, kr);
+  load_v<D, ONCE>(a, head(g), place(t, g), lane, vr);
   const Query<D> q = load_query<D>(a, c, hk, lane & 15, D == 32 ? 32 : 64, D == 32 ? 8 : 16);
   for (; t + STEP < end; t += STEP) {
     const float ks = __shfl(held.ks, 4 * at + g, kWave), vs = __shfl(held.vs, 4 * at + g, kWave);
@@ -810,7 +823,7 @@ __device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, 
     const uint32_t k_head = head(m4), v_head = head(g);
     float4_t acc[4] = {};
     short_scores<D>(kr, q, acc);
-    load_k<D>(a, k_head, place(t + STEP, m4), lane, kr);
+    load_k<D, ONCE>(a, k_head, place(t + STEP, m4), lane, kr);
     half8_t hi[2], lo[2];
     if ((t + 1) * kKeys <= least)
       softmax_tile<D, false>(st, acc, ks, vs, lvs, q.mul, 16, hi, lo);
@@ -818,7 +831,7 @@ __device__ inline void short_tiles(const AttnArgs &a, const Columns &c, int hk, 
       softmax_tile<D, true>(st, acc, ks, vs, lvs, q.mul, min(q.see - t * kKeys, kKeys) - 16 * g, hi,
                             lo);
     short_sums<D>(vr, hi, lo, st);
-    load_v<D>(a, v_head, place(t + STEP, g), lane, vr);
+    load_v<D, ONCE>(a, v_head, place(t + STEP, g), lane, vr);
   }
   // the last tile on its own: a condition on the loads within the loop would have
   // them all waited for
@@ -837,14 +850,14 @@ __device__ inline int end_of(const AttnArgs &a, const Columns &c, int start, int
       min(start + chunk, (seen_by(c.len, c.n, c.base + cols - 1, a.G) + kKeys - 1) / kKeys));
 }
 
-template <int D>
+template <int D, bool ONCE>
 __device__ inline void short_unit(const AttnArgs &a, const Columns &c, const Pick &u, int hk,
                                   int chunk, float *share_at, ShortMem<D> &s) {
   const int tid = thread_here(), lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cols = min(kCols, c.n * a.G - c.base), start = u.range * chunk;
   State<D> st;
-  short_tiles<D, kShortWaves>(a, c, hk, start + wave, end_of(a, c, start, chunk, cols), st);
+  short_tiles<D, kShortWaves, ONCE>(a, c, hk, start + wave, end_of(a, c, start, chunk, cols), st);
   // the four waves' states, then the columns' results or the unit's share of them
   const int col = lane & 15;
   st.l = sum_groups(st.l);
@@ -1167,7 +1180,7 @@ __device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *ti
   while (at < units) {
     const Unit<D, TALL> w(a, find_unit<TALL, WAVES>(a, s, chunk, at / Hkv), at % Hkv, chunk, scratch);
     if (threadIdx.x == 0) s.next = units > gridDim.x ? take_unit(queues) : units;
-    run(w.c, w.u, w.hk, chunk, w.u.ranges > 1 ? w.share_of(w.u.range) : nullptr);
+    run(plan, w.c, w.u, w.hk, chunk, w.u.ranges > 1 ? w.share_of(w.u.range) : nullptr);
     if (w.u.ranges > 1 && last_of(tickets + (int64_t)w.u.ticket * Hkv + w.hk, w.u.ranges, &s.last)) {
       auto share_of = [&](int range) { return w.share_of(range); };
       if constexpr (TALL) {
@@ -1186,6 +1199,16 @@ __device__ inline void run_units(const AttnArgs &a, float *scratch, unsigned *ti
     __syncthreads();                   // the LDS is free
   }
   if (units > gridDim.x && threadIdx.x == 0) leave_queues(queues);
+}
+
+// Whether codes are read once: requests of a group of columns, and more codes than the
+// caches would hold (kept / not kept: 4 requests of up to 131072 tokens, 8 heads of 128
+// dims, 109 / 105 us, 128 of up to 1000 46 / 43, 64 of up to 8000 in blocks of 16 with
+// 64 dims 74 / 68, with 128 dims, though, 136 / 142; with half as many codes 16 of up to
+// 8000, 64 dims, 22.4 / 23.3).
+template <int D>
+__device__ inline bool once_pays(const AttnArgs &a, const Plan &plan) {
+  return (int64_t)a.T * a.G <= (int64_t)kCols * a.B && plan.work * (2 * D * kKeys) * a.p.Hkv > 1e8f;
 }
 
 // Units of 16 columns with a wave each, where there are so many of them that four
@@ -1207,7 +1230,7 @@ __global__ __launch_bounds__(kShortWaves *kWave, 2) void attn_paged_solo_kernel(
                            scratch);
     const int col = thread_here() & 15, start = w.u.range * chunk;
     State<D> st;
-    short_tiles<D, 1>(a, w.c, w.hk, start, end_of(a, w.c, start, chunk, w.cols), st);
+    short_tiles<D, 1, false>(a, w.c, w.hk, start, end_of(a, w.c, start, chunk, w.cols), st);
     wave_end<D>(a, w.c, w.hk, col, w.cols, w.u.ranges,
                 w.u.ranges > 1 ? w.share_of(w.u.range) : nullptr, 0, kCols, st);
     if (w.u.ranges > 1) {
@@ -1230,8 +1253,9 @@ __global__ __launch_bounds__(kShortWaves *kWave, 2) void attn_paged_short_kernel
   __shared__ PlanMem<kShortWaves> s_plan;
   __shared__ __align__(16) union { ShortMem<D> unit; JoinMem join; } s;
   run_units<D, kShort, kShortWaves>(a, scratch, tickets, s_plan, s.join,
-                                   [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
-                                     short_unit<D>(a, c, u, hk, chunk, to, s.unit);
+                                   [&](const Plan &plan, const Columns &c, const Pick &u, int hk, int chunk, float *to) {
+                                     if (once_pays<D>(a, plan)) short_unit<D, true>(a, c, u, hk, chunk, to, s.unit);
+                                     else short_unit<D, false>(a, c, u, hk, chunk, to, s.unit);
                                    });
 }
 
@@ -1241,7 +1265,7 @@ __global__ __launch_bounds__(kTallWaves *kWave, D == 128 ? 2 : 4) void attn_page
   __shared__ PlanMem<kTallWaves> s_plan;
   __shared__ __align__(16) union { TallMem<D> unit; JoinMem join; } s;
   run_units<D, kTall, kTallWaves>(a, scratch, tickets, s_plan, s.join,
-                                 [&](const Columns &c, const Pick &u, int hk, int chunk, float *to) {
+                                 [&](const Plan &plan, const Columns &c, const Pick &u, int hk, int chunk, float *to) {
                                    tall_unit<D>(a, c, u, hk, chunk, to, s.unit);
                                  });
 }
