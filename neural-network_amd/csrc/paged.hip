@@ -513,10 +513,11 @@ __global__ __launch_bounds__(256, 6) void rope_append_paged_kernel(
 // Cached rows as fp32: a wave per 16 rows and head.  Rows whose slots follow one
 // another within 16 tokens of a block are read together: of k a lane takes four
 // codes of a token and writes 16 bytes, of v it takes the 16 tokens of a dim in one
-// load and writes each token's dim beside its neighbours'.  Bound by the writes, four
-// times the codes, and they do not stay in the
-// caches: 24 requests of up to 1000 tokens, 8 heads of 128 dims, 48 us, 4.2 TB/s (61 us
-// with stores that stay).
+// load and writes each token's dim beside its neighbours'.  A workgroup's waves take
+// neighbouring rows of one head, whose tokens of a dim share lines: 24 requests of up
+// to 1000 tokens, 8 heads of 128 dims in blocks of 64, 34 us, 6.0 TB/s, bound by the
+// writes, four times the codes (49 us with the waves on neighbouring heads, and 61
+// with stores that stay in the caches besides).
 constexpr int kReadRows = 16;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -524,9 +525,9 @@ template <int D>
 __global__ __launch_bounds__(256) void kv_read_paged_kernel(
     const int8_t *__restrict__ codes, const float *__restrict__ scales, PagedPool p,
     const int32_t *__restrict__ slots, int T, float *__restrict__ k, float *__restrict__ v) {
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, h = unit % p.Hkv;
-  const int64_t t0 = unit / p.Hkv * kReadRows;
+  // neighbouring rows in a workgroup: their 16 bytes of a dim of v lie side by side
+  const int lane = threadIdx.x & 63, h = blockIdx.x % p.Hkv;
+  const int64_t t0 = ((int64_t)(blockIdx.x / p.Hkv) * 4 + (threadIdx.x >> 6)) * kReadRows;
   if (t0 >= T) return;
   const int mine = lane < kReadRows && t0 + lane < T ? slots[t0 + lane] : -1;
   const int before = __shfl_up(mine, 1, kWave);
@@ -619,8 +620,7 @@ void launch_rope_append_paged(hipStream_t st, const float *qkv, int T, int H, co
 
 void launch_kv_read_paged(hipStream_t st, const int8_t *codes, const float *scales,
                           const PagedPool &p, const int32_t *slots, int T, float *k, float *v) {
-  const int64_t units = ((int64_t)T + kReadRows - 1) / kReadRows * p.Hkv;
-  const dim3 grid((unsigned)((units + 3) / 4));
+  const dim3 grid((unsigned)(((int64_t)T + 4 * kReadRows - 1) / (4 * kReadRows) * p.Hkv));
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, codes, scales, p, slots, T, k, v);
   };
