@@ -11,6 +11,7 @@ namespace nnhip {
 namespace {
 
 constexpr int kWave = 64;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
 // Block tables and slot maps.
@@ -208,7 +209,9 @@ __global__ __launch_bounds__(THREADS) void block_tables_kernel(
 // one after another.  The first quads that a thread has looked at for the scale stay
 // in registers until their codes are stored (more of them cost workgroups a unit:
 // two 22 us, four 27, one 20, where the rest is read from L2 again).  The queries are
-// rotated by workgroups behind those.
+// rotated by workgroups behind those, with stores that do not stay in the caches: on
+// the other dies, which read most of them, they would not be found (with the rows
+// read back 28 us for 32, with attention behind it the same to 1%).
 //
 // 9 prompts of up to 1000 tokens (7835 rows, 16 heads over 4 of 64 dims): 20 us,
 // 4.3 TB/s; bound by memory at that size.  A step of 27 requests: 5 us, latency.
@@ -458,8 +461,8 @@ __global__ __launch_bounds__(256, 6) void rope_append_paged_kernel(
       if (append_slot(a, p, pos, a.slots[t]) < 0) continue;
       double x[4];
       rotate(quad(a, pos, t * stride + (int64_t)(c / D4) * D, c & (D4 - 1), D), x);
-      *reinterpret_cast<float4 *>(q_out + ((int64_t)t * per + c) * 4) =
-          make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+      const f32x4 out = {(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+      __builtin_nontemporal_store(out, reinterpret_cast<f32x4 *>(q_out + ((int64_t)t * per + c) * 4));
     }
     return;
   }
@@ -519,7 +522,6 @@ __global__ __launch_bounds__(256, 6) void rope_append_paged_kernel(
 // writes, four times the codes (49 us with the waves on neighbouring heads, and 61
 // with stores that stay in the caches besides).
 constexpr int kReadRows = 16;
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <int D>
 __global__ __launch_bounds__(256) void kv_read_paged_kernel(
