@@ -458,7 +458,8 @@ int nnhip_rope_kv_append_paged_q8(nnhip_ctx *ctx, const float *qkv, int T,
  * Blocks beyond a request's tokens are not read, tokens that a row does not
  * see have no part in it whatever they hold.  A table entry outside the pool
  * where a token is seen makes the row NaN; lens is cut to max_blocks blocks
- * and row_start to [0, T].  q and out aligned to 16 bytes; B at most 4096; T
+ * and row_start to [0, T] (requests that then have many more rows than T
+ * together have none).  q and out aligned to 16 bytes; B at most 4096; T
  * may be 0.  A row's last bits depend on the batch it is in (the kernel and
  * the split of the keys go by the launch's sizes). */
 int nnhip_attention_paged_q8(nnhip_ctx *ctx, const float *q, int T,

@@ -289,7 +289,7 @@ struct PlanMem {
   // scratch and among the counters
   int upto[WAVES * kWave], slot[WAVES * kWave], ticket[WAVES * kWave];
   int sum[WAVES][3];
-  float work[WAVES];
+  float work[WAVES], groups[WAVES];
   int next, last;
 };
 
@@ -306,44 +306,47 @@ __device__ inline Plan make_plan(const AttnArgs &a, PlanMem<WAVES> &s) {
   const int per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(a.B, b0 + per);
   const Part only = b0 < b1 ? part_of<TALL>(a, b0) : Part{0, 0, 0, 0};
   auto part_at = [&](int b) { return b == b0 ? only : part_of<TALL>(a, b); };
-  // tiles of all groups, from above: fp32 sums are off by 2^-14 at most
-  float work = 0.f;
-  int groups = 0;
+  // tiles of all groups, from above, and groups: fp32 sums are off by 2^-14 at most
+  float work = 0.f, groups = 0.f;
   for (int b = b0; b < b1; ++b) {
     const Part p = part_at(b);
     const float g = (float)p.groups;
     work += TALL ? g * (max(0, p.len - p.n) + 1) / kKeys + g * (g + 1.f) * kTallCols / 2 /
                            (kKeys * (float)a.G) + g
                  : g * (float)tiles_of(p);
-    groups += p.groups;
+    groups += g;
   }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) work += __shfl_xor(work, o, kWave);
-  groups = wave_scan(groups);
-  if (lane == 63) {
+  for (int o = 32; o; o >>= 1) {
+    work += __shfl_xor(work, o, kWave);
+    groups += __shfl_xor(groups, o, kWave);
+  }
+  if (lane == 0) {
     s.work[wave] = work;
-    s.sum[wave][0] = groups;
+    s.groups[wave] = groups;
   }
   __syncthreads();
-  work = 0.f;
-  groups = 0;
+  work = groups = 0.f;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
     work += s.work[w];
-    groups += s.sum[w][0];
+    groups += s.groups[w];
   }
   __syncthreads();
+  // requests that have more rows than there are: counts beyond 32 bits, and no units
+  constexpr int kWide = TALL ? kTallCols : kCols;
+  if (groups > (float)a.T * a.G / kWide * (1.f + 1.f / 1024) + a.B + 1) return Plan{0, 1, 0.f};
   // Short: work / chunk + groups units, all at once.  Tall, solo: no unit longer than
   // a slot's part of the work (the rows of a prompt see more and more tokens).
   const int room = KIND == kSolo ? kSoloSlots
                    : TALL        ? tall_slots(a.p.D)
-                   : groups < kSlots ? max(kShortRoom, kSlots - groups * Hkv)
+                   : groups < kSlots ? max(kShortRoom, kSlots - (int)groups * Hkv)
                                      : kShortRoom;
   const float target = work * (1.f + 1.f / 8192) * Hkv / room;
   // Few long requests: a range costs its own tiles and the join all the ranges'
   // shares, so neither is much longer than the other (one request of 100000 tokens
   // and one head of 64 dims: 30 us in ranges of 8 tiles, 21 in ranges of 29).
-  const int least = KIND == kShort ? max(kShortMin, (int)(0.75f * sqrtf(work / max(groups, 1))))
+  const int least = KIND == kShort ? max(kShortMin, (int)(0.75f * sqrtf(work / fmaxf(groups, 1.f))))
                                    : kTallMin;
   const int chunk = max(least, (int)fminf(target, 1e6f) + 1);
   int mine = 0, shares = 0, shared = 0;      // units, those that share a group, such groups

@@ -217,6 +217,21 @@ def test_nothing_behind_the_tokens_is_seen(ctx, rules, kind):
     assert np.array_equal(first, attend(ctx, c, q, tables, start, lens, H))
 
 
+@pytest.mark.parametrize("kind,T,B,H,Hkv", [("short", 100, 50, 4, 2), ("tall", 800, 6, 32, 2),
+                                            ("solo", 400, 4096, 8, 8), ("tall", 4096, 200, 64, 2)])
+def test_requests_that_have_the_same_rows_have_none(ctx, rules, kind, T, B, H, Hkv):
+    """Bounds that go up and down: half the requests have all of the rows."""
+    D, bs = 32, 16
+    assert kernel(rules, T, B, H, Hkv) == kind
+    c = Cache(ctx, 8, Hkv, D, bs, np.random.default_rng(1))
+    start = np.where(np.arange(B + 1) % 2, T, 0)
+    a = [ctx.array(i32(x)) for x in (np.arange(B * 2).reshape(B, 2) % 8, start, np.full(B, 30))]
+    q, out = (ctx.array(np.full((T, H * D), x, np.float32)) for x in (1, 7))
+    nnhip.call("nnhip_attention_paged_q8", ctx.h, q.p, T, c.dc.p, c.ds.p, bs, c.blocks, a[0].p, 2,
+               a[1].p, a[2].p, B, H, Hkv, D, out.p)
+    assert (out.numpy() == 7).all()
+
+
 @pytest.mark.parametrize("kind", ["tall", "solo"])
 @pytest.mark.parametrize("kv", [0, 1])
 def test_a_block_whose_scale_is_no_number(ctx, rules, kind, kv):
