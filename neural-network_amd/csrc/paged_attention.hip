@@ -234,7 +234,7 @@ struct Ranges {
 
   __device__ Ranges(const Part &p, int chunk_, int G_)
       : chunk(chunk_), groups(p.groups), past((int64_t)p.len - p.n), G(G_) {
-    count = max(1, (tiles_of(p) + chunk - 1) / chunk);
+    count = groups ? max(1, (tiles_of(p) + chunk - 1) / chunk) : 1;
     shared = count > 1 ? first_group(1) : groups;
   }
   __device__ int first_group(int s) const {

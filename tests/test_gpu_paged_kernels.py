@@ -84,6 +84,28 @@ def test_wide_units_of_several_ranges(ctx, rules, D):
     check_rows(got, c, q, tables, start, lens, H, sample(np.random.default_rng(2), start, 2))
 
 
+def test_long_requests_without_rows_beside_prompts(ctx, rules):
+    """They have no ranges to count, however long they are."""
+    counts, lens = [900, 0, 0, 700, 0], [930, 2 ** 30, 2 ** 30, 700, 5000]
+    rng = np.random.default_rng(28)
+    mb = 2 ** 30 // 128
+    tables = np.zeros((5, 64), np.int64)
+    tables[0, :8], tables[3, :6] = rng.permutation(20)[:8], rng.permutation(20)[:6]
+    c = Cache(ctx, 20, 2, 64, 128, rng)
+    start = np.concatenate(([0], np.cumsum(counts)))
+    q = rng.standard_normal((1600, 16 * 64)).astype(np.float32)
+    assert kernel(rules, 1600, 5, 16, 2) == "tall"
+    wide = ctx.array(shape=(5, mb), dtype=np.int32)     # rows of 2^23 entries
+    flat = np.zeros((5, mb), np.int32)
+    flat[:, :64] = tables
+    wide.upload(flat)
+    a = [ctx.array(x) for x in (q, i32(start), i32(lens))]
+    out = ctx.array(np.full((1600, 16 * 64), 7.0, np.float32))
+    nnhip.call("nnhip_attention_paged_q8", ctx.h, a[0].p, 1600, c.dc.p, c.ds.p, 128, 20, wide.p, mb,
+               a[1].p, a[2].p, 5, 16, 2, 64, out.p)
+    check_rows(out.numpy(), c, q, tables, start, lens, 16, sample(rng, start, 3))
+
+
 def test_wide_units_that_see_nothing(ctx, rules):
     """More rows than tokens: the first of them are zero."""
     counts, lens = [800, 700, 400], [30, 700, 0]
