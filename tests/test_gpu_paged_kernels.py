@@ -163,6 +163,35 @@ def test_narrow_units_in_queues(ctx, rules, D):
     check_rows(got, c, q, tables, start, list(lens), 16, rows)
 
 
+@pytest.mark.parametrize("B", [63, 64, 65])
+@pytest.mark.parametrize("D", [64, 128])
+def test_as_many_requests_as_a_wave_has_lanes(ctx, rules, B, D):
+    """And one more: the plan is a wave's or the workgroup's.  Units in queues, some
+    requests without rows or tokens, the last with several ranges."""
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, 100, B)
+    lens[[1, B - 1]] = 3000, 1300
+    counts = np.minimum(1 + (np.arange(B) % 5 != 2), lens)
+    counts[[7, 30]] = 0
+    c, q, tables, start = problem(ctx, D, list(lens), list(counts), 16, 16, D, 32, pad=2)
+    assert kernel(rules, len(q), B, 16, 16) == "short" and B * 16 > 512
+    got = attend(ctx, c, q, tables, start, list(lens), 16)
+    assert (got[start[-1]:] == 7).all()
+    check_rows(got, c, q, tables, start, list(lens), 16, range(0, start[-1], 3))
+
+
+@pytest.mark.parametrize("B", [64, 70])
+def test_wide_units_of_many_requests(ctx, rules, B):
+    rng = np.random.default_rng(B)
+    counts = rng.integers(0, 60, B)
+    lens = counts + rng.integers(0, 90, B)
+    lens[5] += 2500
+    c, q, tables, start = problem(ctx, 1, list(lens), list(counts), 32, 4, 64, 16, pad=1)
+    assert kernel(rules, len(q), B, 32, 4) == "tall"
+    got = attend(ctx, c, q, tables, start, list(lens), 32)
+    check_rows(got, c, q, tables, start, list(lens), 32, sample(rng, start, 1))
+
+
 def test_calls_of_all_kinds_follow_one_another(ctx, rules):
     """Counters and scratch that a context keeps are left as the next call needs
     them: the same bits again, whatever ran before, also by turns with a context of
