@@ -72,18 +72,18 @@ inline bool attention_prompt_shape(int B, int S, int H, int D, bool q8, int max_
 // request, or of 16.  The wide ones read each key and value for eight times as many
 // columns, but a unit that a request does not fill costs as much as a full one, and
 // few units leave the card idle.  16 heads over 4, wide / narrow: 4 prompts of up to
-// 800 rows of 128 dims 43 / 62 us (36 / 41 of 64 dims), of up to 200 rows 18 / 20;
-// 400 rows behind up to 2000 tokens 78 / 77, 200 rows 57 / 40; 2 chunks of 500 rows
-// beside 33 requests that decode 79 / 66, beside 100 119 / 82.
+// 800 rows of 128 dims 40 / 61 us (34 / 43 of 64 dims), of up to 200 rows 16 / 19;
+// 400 rows behind up to 2000 tokens 71 / 73, 200 rows 52 / 39; 2 chunks of 500 rows
+// beside 31 requests that decode 71 / 63, beside 98 105 / 84.
 inline bool attention_paged_tall(int T, int B, int G, int Hkv) {
   return (int64_t)T * G >= (int64_t)128 * B && (int64_t)T * G * Hkv >= 24576;
 }
 
 // Units of 16 columns, with a wave each or with four: `groups` estimates how many
 // there are.  A wave each saves the join of four states, four share a long context.
-// One / four: 512 requests of up to 300 tokens, 4 heads of 128 dims 31 / 41 us, 16 of
-// 64 dims 55 / 90; 128 of up to 1000, 8 heads of 64 dims, 35 / 26, of up to 100, 128
-// dims, 16 / 19.
+// One / four: 512 requests of up to 300 tokens, 4 heads of 128 dims 32 / 41 us, 16 of
+// 64 dims 55 / 89; 128 of up to 1000, 8 heads of 64 dims, 33 / 26, of up to 100, 128
+// dims, 15 / 19; 4 prompts of up to 400 rows behind up to 2000 tokens 53 / 48.
 inline bool attention_paged_solo(int T, int B, int G, int Hkv) {
   const int64_t groups = std::max<int64_t>(((int64_t)T * G + 15) / 16, std::min(T, B));
   return groups * Hkv >= 1536 && (int64_t)T * G < (int64_t)32 * B;
